@@ -14,6 +14,42 @@ LIB_PATH = os.environ.get("GRADTTS_LIB", os.path.join(_HERE, "libgradtts.so"))
 
 GT_OK, GT_ERR_ARG, GT_ERR_HIP, GT_ERR_PARAM, GT_ERR_UNSUPPORTED, GT_ERR_WORKSPACE = range(6)
 GT_F32, GT_BF16, GT_BF16_W8, GT_FP8 = 0, 1, 2, 3
+GT_ELEM_F32, GT_ELEM_BF16, GT_ELEM_F16 = 0, 1, 2
+
+
+class Stride(ctypes.Structure):
+    """gt_stride (include/gradtts.h)"""
+    _fields_ = [("b", ctypes.c_int64), ("t", ctypes.c_int64), ("h", ctypes.c_int64)]
+
+
+class BucketAttention(ctypes.Structure):
+    """gt_bucket_attention"""
+    _fields_ = ([(n, ctypes.c_int32) for n in ("dtype", "causal", "n_buckets", "max_distance")] +
+                [("scale", ctypes.c_float)] + [(n, ctypes.c_int64) for n in ("B", "Tq", "Tk", "Hq", "Hkv", "D")] +
+                [(n, ctypes.c_void_p) for n in ("q", "k", "v", "table")] +
+                [(n, Stride) for n in ("q_stride", "k_stride", "v_stride", "out_stride")] +
+                [(n, ctypes.c_void_p) for n in ("lengths", "q_lengths", "q_start")])
+
+
+class BucketAttentionGrads(ctypes.Structure):
+    """gt_bucket_attention_grads"""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("dout", "dq", "dk", "dv", "dtable")] +
+                [(n, Stride) for n in ("dout_stride", "dq_stride", "dk_stride", "dv_stride")])
+
+
+class ResidualNorm(ctypes.Structure):
+    """gt_residual_norm"""
+    _fields_ = ([(n, ctypes.c_int32) for n in ("dtype", "rms", "gate_per_batch")] +
+                [(n, ctypes.c_float) for n in ("scale", "eps")] + [(n, ctypes.c_int64) for n in ("B", "T", "C")] +
+                [(n, ctypes.c_void_p) for n in ("x", "y", "gate", "post_weight", "post_bias", "pre_weight", "pre_bias",
+                                                "lengths")])
+
+
+class ResidualNormGrads(ctypes.Structure):
+    """gt_residual_norm_grads"""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("dout", "dh", "dx", "dy", "dgate", "dpost_weight", "dpost_bias",
+                                               "dpre_weight", "dpre_bias")]
+
 
 # (name, restype, argtypes) for every symbol declared in include/gradtts.h
 _c = ctypes
@@ -107,6 +143,14 @@ SIGNATURES = [
     ("gt_vocoder_workspace_bytes", _c.c_size_t, [_c.c_void_p, _c.c_int64, _c.c_int64]),
     ("gt_vocoder_forward", _c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_void_p,
                                       _c.c_size_t, _c.c_void_p]),
+    ("gt_relative_bucket", _c.c_int, [_c.c_int, _c.c_int, _c.c_int, _c.c_int64]),
+    ("gt_bucket_attention_workspace_bytes", _c.c_size_t, [_c.c_void_p]),
+    ("gt_bucket_attention_forward", _c.c_int, [_c.c_void_p] * 4 + [_c.c_size_t, _c.c_void_p]),
+    ("gt_bucket_attention_backward_workspace_bytes", _c.c_size_t, [_c.c_void_p]),
+    ("gt_bucket_attention_backward", _c.c_int, [_c.c_void_p] * 5 + [_c.c_size_t, _c.c_void_p]),
+    ("gt_residual_norm_forward", _c.c_int, [_c.c_void_p] * 5),
+    ("gt_residual_norm_backward_workspace_bytes", _c.c_size_t, [_c.c_void_p]),
+    ("gt_residual_norm_backward", _c.c_int, [_c.c_void_p] * 4 + [_c.c_size_t, _c.c_void_p]),
     ("gt_alignment_workspace_bytes", _c.c_size_t, [_c.c_int64, _c.c_int64, _c.c_int64]),
     ("gt_log_prior_maximum_path", _c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int64,
                                              _c.c_int64, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_void_p,

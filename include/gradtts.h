@@ -316,6 +316,75 @@ int gt_maximum_path(int32_t* paths, const float* values, const int32_t* t_xs, co
                     int64_t tx_max, int64_t ty_max, float max_neg_val, void* workspace, size_t workspace_bytes,
                     void* stream);
 
+/* ---- Operators of transformer blocks ----
+ * Element types of their tensors (parameters of the residual step are fp32 throughout). */
+enum { GT_ELEM_F32 = 0, GT_ELEM_BF16 = 1, GT_ELEM_F16 = 2 };
+typedef struct { int64_t b, t, h; } gt_stride;   /* elements from one batch entry / position / head to the next */
+
+/* Attention with a learned relative position bias by buckets:
+ *   out[b,i,h] = sum_j softmax_j(q[b,i,h] . k[b,j,h'] scale + table[bucket(j - pos_i)][h]) v[b,j,h'],
+ *   pos_i = q_start[b] + i, h' = h / (Hq / Hkv); q, out [B,Tq,Hq,D], k, v [B,Tk,Hkv,D] by their strides (channels
+ *   contiguous), table [n_buckets][Hq] contiguous, all of one element type; 1 <= D <= 128, Hq a multiple of Hkv.
+ * Buckets of one direction: n = n_buckets if causal (distance max(pos_i - j, 0); keys j > pos_i are not seen), else
+ * n_buckets / 2 (distance |j - pos_i|; offsets j > pos_i use the second n). Distances below exact = n / 2 have a bucket
+ * each; distance d >= exact has exact + min(n - exact - 1, floor((n - exact) log(d / exact) / log(max_distance /
+ * exact))), borders exact in whole numbers. 2 <= n_buckets <= 128 (bidirectional: even, >= 4), exact < max_distance <=
+ * 1024. scale in [2^-20, 2^20].
+ * lengths [B]: keys j >= lengths[b] are not seen, nor read (NULL: all of Tk). q_lengths [B]: rows i >= q_lengths[b]
+ * give zeros and take no gradient (NULL: all). q_start [B] (NULL: 0). Rows that see no key give zeros. lengths are
+ * clamped to [0, Tk] / [0, Tq].
+ * lse: NULL, or [B,Hq,Tq] fp32 for the backward: log2 of the row's sum of exponentials (+inf: no key).
+ * backward: writes dq, dk, dv (any strides, channels contiguous) and dtable [n_buckets][Hq] from the forward's
+ * arguments, its out and lse, and dout. Every sum runs in a fixed order: results repeat bit for bit.
+ * gt_relative_bucket: the bucket of offset j - pos_i (host; -1: arguments outside the ranges above). */
+typedef struct {
+  int32_t dtype, causal, n_buckets, max_distance;
+  float scale;
+  int64_t B, Tq, Tk, Hq, Hkv, D;
+  const void *q, *k, *v, *table;
+  gt_stride q_stride, k_stride, v_stride, out_stride;
+  const int64_t *lengths, *q_lengths, *q_start;
+} gt_bucket_attention;
+typedef struct {
+  const void* dout;
+  void *dq, *dk, *dv, *dtable;
+  gt_stride dout_stride, dq_stride, dk_stride, dv_stride;
+} gt_bucket_attention_grads;
+int gt_relative_bucket(int causal, int n_buckets, int max_distance, int64_t offset);
+size_t gt_bucket_attention_workspace_bytes(const gt_bucket_attention* a);
+int gt_bucket_attention_forward(const gt_bucket_attention* a, void* out, float* lse, void* workspace,
+                                size_t workspace_bytes, void* stream);
+size_t gt_bucket_attention_backward_workspace_bytes(const gt_bucket_attention* a);
+int gt_bucket_attention_backward(const gt_bucket_attention* a, const void* out, const float* lse,
+                                 const gt_bucket_attention_grads* g, void* workspace, size_t workspace_bytes,
+                                 void* stream);
+
+/* The residual step between two blocks with norms on both sides of a block:
+ *   out = x + scale gate N1(y),  h = N2(out),  N(t) = u w + b over the C channels,
+ *   u = (t - mean) / sqrt(var + eps), or t / sqrt(mean(t^2) + eps) with rms = 1;
+ * x, y, out, h [B,T,C] contiguous of one element type; gate [C], or [B,C] with gate_per_batch, or NULL (1); weights
+ * and biases [C] (biases may be NULL); all parameters fp32. C <= 8192. lengths [B]: rows t >= lengths[b] are not read,
+ * their outputs and gradients are zero (NULL: all of T). stats: NULL, or [B,T,4] fp32 for the backward.
+ * backward: from the forward's arguments, its stats, dout and dh: dx, dy [B,T,C] and the parameters' fp32 gradients
+ * (those of absent parameters must be NULL; dgate has the gate's shape). Fixed summation order. */
+typedef struct {
+  int32_t dtype, rms, gate_per_batch;
+  float scale, eps;
+  int64_t B, T, C;
+  const void *x, *y;
+  const float *gate, *post_weight, *post_bias, *pre_weight, *pre_bias;
+  const int64_t* lengths;
+} gt_residual_norm;
+typedef struct {
+  const void *dout, *dh;
+  void *dx, *dy;
+  float *dgate, *dpost_weight, *dpost_bias, *dpre_weight, *dpre_bias;
+} gt_residual_norm_grads;
+int gt_residual_norm_forward(const gt_residual_norm* a, void* out, void* h, float* stats, void* stream);
+size_t gt_residual_norm_backward_workspace_bytes(const gt_residual_norm* a);
+int gt_residual_norm_backward(const gt_residual_norm* a, const float* stats, const gt_residual_norm_grads* g,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
