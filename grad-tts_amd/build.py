@@ -23,7 +23,7 @@ OPS_OUT = os.path.join(HERE, "gradtts_amd", "libgradtts_ops.so")   # torch.ops.g
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = os.environ.get("GRADTTS_ARCH", "gfx950")
 SOURCES = ["conv.hip", "conv1s.hip", "conv64.hip", "conv3w.hip", "conv3w_a8.hip", "attn.hip", "attn_down.hip", "misc.hip", "mas.hip", "train.hip", "bwd.hip", "textenc.hip", "textenc_train.hip",
-           "battn.hip", "rnorm.hip", "decoder.cpp", "train_bwd.cpp", "textenc.cpp", "vocoder.cpp", "block_ops.cpp"]
+           "battn_fwd.hip", "battn_bwd.hip", "rnorm.hip", "decoder.cpp", "train_bwd.cpp", "textenc.cpp", "vocoder.cpp", "block_ops.cpp"]
 # -packed-fp32-ops: keep the compiler from emitting v_pk_{fma,add,mul}_f32. Rounds 1-2 saw run-to-run differences
 # with them (GroupNorm sum-of-squares partials, W8 decodes); round 3 found the cause -- the compiler paired the
 # per-lane GroupNorm sum / sum-of-squares chains into packed ops whose op_sel_hi read a dword the previous VALU

@@ -1,4 +1,4 @@
-// Attention with a learned relative position bias by buckets (battn.hip): parameter block and launchers.
+// Attention with a learned relative position bias by buckets (battn_fwd.hip, battn_bwd.hip): parameter block, launchers.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -20,16 +20,19 @@ struct BaParams {
   int nb, side, exact, nborder, dsat;
   int border[63];
   const int64_t *len, *qlen, *qstart;   // [B] or null: all of Tk, all of Tq, 0
+  int ntile, zigzag;                 // tiles of the launch's stationary side and their order (tile_of)
   // forward
   void* out; BaStride os;
   float* lse;                        // [B][Hq][Tq], log2 units; +inf: no visible key
-  // split form
-  int nsplit, split_keys;            // keys a split covers
-  float* part;                       // [B][Hkv][row blocks][nsplit][32][DP + 2]
+  int gp, qpb;                       // spread form: heads and queries packed into the 32 rows of a block
+  int nsplit, split_keys;            // spread form: key ranges of their own workgroups
+  float *part, *part_ml;             // [row block][split][32][D]; [row block][split][2][32]
   // backward
   const void *o, *dout; BaStride dos;
   void *dq, *dk, *dv, *dtable; BaStride dqs, dks, dvs;
-  float *delta, *tpart;              // [B][Hq][Tq]; [nb][Hq][B * q tiles]
+  float *delta, *tpart;              // [B][Hq][Tq]; [nb][Hq][B ntile]
+  int gsplit;                        // dK dV: groups of heads with workgroups of their own, summed from gpart
+  float* gpart;                      // [2][gsplit][B][Tk][Hkv][D]
 };
 
 // dtype: 0 fp32, 1 bf16, 2 fp16

@@ -1,0 +1,505 @@
+// Attention with a learned relative position bias by buckets, gfx950, backward:
+//   P = 2^(scores - lse),  dP = dO V^T,  delta = rowsum(P o dP) (= rowsum(o o dO)),  dS = P o (dP - delta)
+//   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO,  dtable[c][h] = sum of dS over the pairs of bucket c
+// Two kernels, each the sole writer of its rows, so that every sum has one order: dQ (with delta and the table's
+// partial sums) streams keys past 32-row query blocks, dK dV streams queries past key blocks. Scores and dP are formed
+// in both: 7 products instead of 5, against atomics or a T x T matrix in memory.
+#include "battn_core.h"
+
+namespace gt {
+namespace {
+
+// Sums over the diagonals of a 32 x 32 block (rows: registers and lane half, columns: lane & 31): lane i of the result
+// has those with row - column = 31 - i. Rows in ascending order, the running sums moving up a lane before each row:
+// one add with a lane shift (v_add_f32, wave_shr:1) a row.
+GT_DEV float diagonals(const float (&x)[16]) {
+  float a = 0.f;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    float lo[4], hi[4];   // rows 8 g + e and 8 g + 4 + e in lanes 0 .. 31, zeros above
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(x[4 * g + e]), 0u, false, false);
+      lo[e] = __uint_as_float(w[0]);
+      hi[e] = __uint_as_float(w[1]);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float up = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(a), 0x138, 0xf, 0xf, true));
+      a = up + (e < 4 ? lo[e & 3] : hi[e & 3]);
+    }
+  }
+  return a;
+}
+
+// ================================================================ dQ, delta, table partials
+// The product o . do with the rounded o, formed from rounded P, is off by about u |o| |do| (u = half a step of the
+// type), which weighs when few keys share a row: dS = P (dP - delta) is then a small difference. Rows whose keys all lie
+// in the first tile therefore sum P dP itself in fp32 (both are at hand; bf16, 14 keys: dq's error 2.5e-3 where the
+// product's gave 5.4e-3). The others take the product, from the matrix cores in the channel order of dP: so does a row
+// with one visible key (o = v), whose delta then equals dP bit for bit and whose dS is exactly zero.
+template <class T, int DP, int WR, int WS>
+__global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 ? 1 : 2) void ba_dq_kernel(BaParams p) {
+  typedef Tile<T, DP> TL;
+  typedef typename El<T>::frag frag;
+  typedef Shape<T, DP, WS> SH;
+  constexpr int KT = SH::KT, NB = SH::NB, KS = DP / 16, DB = DP / 32, NT = 64 * WR * WS, NW = WR * WS;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int elen = ext_len(p);
+  float* ext0 = (float*)(smem + SH::BYTES);
+  const float* ext = ext0 + p.dsat + EXT;
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wv % WR, ws = wv / WR;
+  const int r = lane & 31, hh = lane >> 5;
+  float* tacc = ext0 + (1 + wv) * elen + p.dsat + EXT;   // this wave's sums of dS by offset
+  float* sat = ext0 + (1 + NW) * elen;                   // [NW][2]; [WS][32] before
+  const int nbk = p.B * p.Hkv, bk = blockIdx.x % nbk, rest = blockIdx.x / nbk, b = bk / p.Hkv, hk = bk % p.Hkv;
+  const int h = hk * p.G + rest % p.G, tl = tile_of(rest / p.G, p.ntile, p.zigzag);
+  const int qlen = clamp_len(p.qlen, b, p.Tq), klen = clamp_len(p.len, b, p.Tk), pos0 = start_of(p, b);
+  const int q0 = tl * 32 * WR, wq0 = q0 + 32 * wr, qi = wq0 + r;
+  int kend = klen;
+  if (p.causal) kend = min(kend, pos0 + min(q0 + 32 * WR, qlen));
+  if (q0 >= qlen) kend = 0;
+  const T* kb = (const T*)p.k + b * p.ks.b + hk * p.ks.h;
+  const T* vb = (const T*)p.v + b * p.vs.b + hk * p.vs.h;
+  auto tile = [&](int t, int which) { return smem + ((SH::NBUF == 2 ? t & 1 : 0) * 2 + which) * SH::TILE; };
+  auto load = [&](int t) {
+    stage<T, DP, KT, NT>(tile(t, 0), kb, p.ks.t, t * KT, klen, p.D, p.vec, tid);
+    stage<T, DP, KT, NT>(tile(t, 1), vb, p.vs.t, t * KT, klen, p.D, p.vec, tid);
+  };
+  const int ntile = kend > 0 ? (kend + KT - 1) / KT : 0;
+  if (ntile && SH::NBUF == 2) load(0);
+  const long srow = ((long)b * p.Hq + h) * p.Tq + qi;
+  const bool in = qi < qlen;
+  frag qf[KS], gf[KS];
+  float delta = 0.f;
+  {
+    const T* qb = (const T*)p.q + b * p.qs.b + h * p.qs.h + (long)qi * p.qs.t;
+    const T* ob = (const T*)p.o + b * p.os.b + h * p.os.h + (long)qi * p.os.t;
+    const T* gb = (const T*)p.dout + b * p.dos.b + h * p.dos.h + (long)qi * p.dos.t;
+    f32x16 dg;
+    zero16(dg);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      qf[s] = in ? load_row8(qb, 16 * s + 8 * hh, p.D, p.vec) : El<T>::zero();
+      gf[s] = in ? load_row8(gb, 16 * s + 8 * hh, p.D, p.vec) : El<T>::zero();
+      const frag of = in ? load_row8(ob, 16 * s + 8 * hh, p.D, p.vec) : El<T>::zero();
+      El<T>::mma(of, gf[s], dg);
+    }
+    // the diagonal: row r of column r, held by lane half (r >> 2) & 1 in register (r & 3) + 4 (r >> 3)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) delta = acc_row(j, hh) == r ? dg[j] : delta;
+    float a, c;
+    halves(delta, a, c);
+    delta = ((r >> 2) & 1) ? c : a;
+  }
+  const float lse = in ? p.lse[srow] : kInf;
+  for (int i = tid; i < NW * elen; i += NT) ext0[elen + i] = 0.f;
+  if (ntile) {
+    if (p.vec && p.D < DP)
+      for (int i = 0; i < 2 * SH::NBUF; ++i) clear_pad<T, DP>(smem + i * SH::TILE, KT, p.D, tid, NT);
+    build_ext<T>(p, h, ext0, tid, NT);
+  }
+  const float blo = table_at<T>(p, p.side - 1, h) * kLog2e, bhi = p.causal ? 0.f : table_at<T>(p, 2 * p.side - 1, h) * kLog2e;
+  f32x16 dq[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) zero16(dq[d]);
+  float slo = 0.f, shi = 0.f;   // dS beyond the last border
+  const int pos = pos0 + qi, pmin = pos0 + wq0, pmax = pmin + 31;
+  const int nkey = p.causal ? min(klen, pos + 1) : klen;                       // keys this lane's row sees
+  const int wend = wq0 >= qlen ? 0 : p.causal ? min(kend, pmax + 1) : kend;    // keys this wave looks at
+  // P and dP of the 32 keys from kk on (block j2 of the tile); unseen keys: 0
+  auto probs = [&](const char* sk, const char* sv, int kk, int j2, float (&pr)[16], f32x16& dp) {
+    const int dmax = kk + 31 - pmin, dmin = kk - pmax;
+    f32x16 s;
+    float off = 0.f;
+    zero16(dp);
+    if (dmax <= -p.dsat) { off = blo; zero16(s); }
+    else if (!p.causal && dmin >= p.dsat) { off = bhi; zero16(s); }
+    else {
+      const float* e = ext + (kk + 4 * hh - pos);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) s[j] = e[acc_row(j, 0)];
+    }
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      El<T>::mma(TL::row(sk, 32 * j2 + r, 2 * ks + hh), qf[ks], s);
+      El<T>::mma(TL::row(sv, 32 * j2 + r, 2 * ks + hh), gf[ks], dp);
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) pr[j] = expo<T>(s[j], p.c, off, lse);
+    if (kk + 31 >= klen || (p.causal && dmax > 0)) {
+      const int lim = nkey - kk - 4 * hh;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) pr[j] = acc_row(j, 0) < lim ? pr[j] : 0.f;
+    }
+  };
+  for (int t = 0; t < ntile; ++t) {
+    if constexpr (SH::NBUF == 2) {
+      lds_ready();
+      if (t + 1 < ntile) load(t + 1);
+    } else {
+      __syncthreads();
+      load(t);
+      lds_ready();
+    }
+    const char *sk = tile(t, 0), *sv = tile(t, 1);
+    if (t == 0 && (WS > 1 ? kend : wend) <= KT) {
+      float sum = 0.f;
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const int kk = 32 * (ws + WS * n);
+        if (kk >= wend) break;
+        float pr[16];
+        f32x16 dp;
+        probs(sk, sv, kk, ws + WS * n, pr, dp);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sum = acc_row(j, hh) + kk < nkey ? __builtin_fmaf(pr[j], dp[j], sum) : sum;
+      }
+      sum = both_sum(sum);
+      if constexpr (WS > 1) {   // all of the workgroup is here: its keys all lie in this tile
+        if (hh == 0) sat[32 * ws + r] = sum;
+        __syncthreads();
+        sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < WS; ++w) sum += sat[32 * w + r];
+      }
+      if (nkey > 1) delta = sum;
+    }
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const int j2 = ws + WS * n, kk = t * KT + 32 * j2;
+      if (kk >= wend) break;
+      const int dmax = kk + 31 - pmin, dmin = kk - pmax;
+      float ds[16];
+      f32x16 dp;
+      probs(sk, sv, kk, j2, ds, dp);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) ds[j] *= dp[j] - delta;
+      if (dmax <= -p.dsat || (!p.causal && dmin >= p.dsat)) {
+        float a = 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) a += ds[j];
+        if (dmin < 0) slo += a;
+        else shi += a;
+      } else {
+        const float a = diagonals(ds);   // lane i: offset kk - pmin + 31 - i
+        if (lane < 63)                   // one add an offset and block, this wave's own array: one order
+          __hip_atomic_fetch_add(tacc + (kk - pmin + 31 - lane), a, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      }
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt) {
+        const frag df = El<T>::pack(ds + 8 * tt);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) El<T>::mma(TL::col(sk, 32 * j2 + 16 * tt, d, lane), df, dq[d]);
+      }
+    }
+  }
+  if (qi < p.Tq && hh == 0 && ws == 0) p.delta[srow] = in ? delta : 0.f;
+  if constexpr (WS == 1) {
+    if (qi < p.Tq) {
+      T* qo = (T*)p.dq + b * p.dqs.b + h * p.dqs.h + (long)qi * p.dqs.t;
+      if (in) store_rows<T, DP>(qo, dq, p.scale, p.D, p.vec, hh);
+      else zero_rows<T, DP>(qo, p.D, p.vec, hh);
+    }
+  } else {
+    join<DP, WS>(smem, dq, p.scale, ws, lane, tid, [&](int row, int d, float* x) {
+      const int i = q0 + row;
+      if (i >= p.Tq) return;
+      if (!(i < qlen)) x[0] = x[1] = x[2] = x[3] = 0.f;
+      store4_row((T*)p.dq + b * p.dqs.b + h * p.dqs.h + (long)i * p.dqs.t, d, x, p.D, p.vec);
+    });
+  }
+  // table partials of this tile: a wave a bucket, its lanes over the bucket's offsets, then across the lanes in one order
+#pragma unroll
+  for (int x = 32; x > 0; x >>= 1) {
+    slo += __shfl_xor(slo, x);
+    shi += __shfl_xor(shi, x);
+  }
+  __syncthreads();
+  if (lane == 0) { sat[2 * wv] = slo; sat[2 * wv + 1] = shi; }
+  __syncthreads();
+  const long npart = (long)p.B * p.ntile;
+  for (int c = wv; c < p.nb; c += NW) {
+    const int side = c >= p.side, cc = side ? c - p.side : c;
+    int d0, d1;   // distances of the bucket
+    if (cc < p.exact) {
+      d0 = cc;
+      d1 = cc + 1;
+    } else {
+      d0 = cc == p.exact ? p.exact : p.border[cc - p.exact - 1];
+      d1 = cc == p.side - 1 ? p.dsat + EXT + 1 : p.border[cc - p.exact];
+    }
+    if (side && d0 == 0) d0 = 1;   // offset 0 belongs to the first half
+    float a = 0.f;
+    for (int d = d0 + lane; d < d1; d += 64)
+#pragma unroll
+      for (int w = 0; w < NW; ++w) a += ext0[(1 + w) * elen + p.dsat + EXT + (side ? d : -d)];
+#pragma unroll
+    for (int x = 32; x > 0; x >>= 1) a += __shfl_xor(a, x);
+    if (cc == p.side - 1)
+      for (int w = 0; w < NW; ++w) a += sat[2 * w + side];
+    if (lane == 0) p.tpart[((long)c * p.Hq + h) * npart + (long)b * p.ntile + tl] = a;
+  }
+}
+
+template <class T> __global__ __launch_bounds__(64) void ba_dtable_kernel(const float* part, long npart, T* dtable) {
+  const float* x = part + (long)blockIdx.x * npart;
+  float a = 0.f;
+  for (long i = threadIdx.x; i < npart; i += 64) a += x[i];
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) a += __shfl_xor(a, s);
+  if (threadIdx.x == 0) dtable[blockIdx.x] = (T)a;
+}
+
+// ================================================================ dK, dV
+// 32 WR keys of one key / value head over the query tiles of the heads that share it, or, where that leaves CUs idle, of
+// a part of them (gsplit), summed afterwards in fp32.
+template <class T, int DP, int WR, int WS>
+__global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 || DP > 96 ? 1 : 2) void ba_dkv_kernel(BaParams p) {
+  typedef Tile<T, DP> TL;
+  typedef typename El<T>::frag frag;
+  typedef Shape<T, DP, WS> SH;
+  constexpr int QT = SH::KT, NB = SH::NB, KS = DP / 16, DB = DP / 32, NT = 64 * WR * WS;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  float* stat = (float*)(smem + SH::BYTES);   // [NBUF][2][QT]: lse, delta of the tile's rows
+  float* ext0 = stat + SH::NBUF * 2 * QT;
+  const float* ext = ext0 + p.dsat + EXT;
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wv % WR, ws = wv / WR;
+  const int r = lane & 31, hh = lane >> 5;
+  const int nbk = p.B * p.Hkv, bk = blockIdx.x % nbk, rest = blockIdx.x / nbk, b = bk / p.Hkv, hk = bk % p.Hkv;
+  // the first key tiles have the most queries under a causal mask
+  const int gs = rest % p.gsplit, tl = p.ntile - 1 - tile_of(rest / p.gsplit, p.ntile, p.zigzag);
+  const int k0 = tl * 32 * WR, wk0 = k0 + 32 * wr, ki = wk0 + r;
+  const int qlen = clamp_len(p.qlen, b, p.Tq), klen = clamp_len(p.len, b, p.Tk), pos0 = start_of(p, b);
+  const int qbeg = (p.causal ? max(0, k0 - pos0) : 0) / QT * QT;   // first tile with a query that sees key k0
+  const int qend = k0 < klen ? qlen : 0;
+  const T* kb = (const T*)p.k + b * p.ks.b + hk * p.ks.h + (long)ki * p.ks.t;
+  const T* vb = (const T*)p.v + b * p.vs.b + hk * p.vs.h + (long)ki * p.vs.t;
+  const bool in = ki < klen;
+  f32x16 dk[DB], dv[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) { zero16(dk[d]); zero16(dv[d]); }
+  if (qbeg < qend) {
+    frag kf[KS], vf[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      kf[s] = in ? load_row8(kb, 16 * s + 8 * hh, p.D, p.vec) : El<T>::zero();
+      vf[s] = in ? load_row8(vb, 16 * s + 8 * hh, p.D, p.vec) : El<T>::zero();
+    }
+    if (p.vec && p.D < DP)
+      for (int i = 0; i < 2 * SH::NBUF; ++i) clear_pad<T, DP>(smem + i * SH::TILE, QT, p.D, tid, NT);
+    const int ntile = (qend - qbeg + QT - 1) / QT, hper = p.G / p.gsplit;
+    for (int g = 0; g < hper; ++g) {
+      const int h = hk * p.G + gs * hper + g;
+      const T* qb = (const T*)p.q + b * p.qs.b + h * p.qs.h;
+      const T* gb = (const T*)p.dout + b * p.dos.b + h * p.dos.h;
+      const float* lse = p.lse + ((long)b * p.Hq + h) * p.Tq;
+      const float* del = p.delta + ((long)b * p.Hq + h) * p.Tq;
+      auto tile = [&](int t, int which) { return smem + ((SH::NBUF == 2 ? t & 1 : 0) * 2 + which) * SH::TILE; };
+      auto stats = [&](int t) { return stat + (SH::NBUF == 2 ? t & 1 : 0) * 2 * QT; };
+      auto load = [&](int t) {
+        const int q0 = qbeg + t * QT;
+        stage<T, DP, QT, NT>(tile(t, 0), qb, p.qs.t, q0, qlen, p.D, p.vec, tid);
+        stage<T, DP, QT, NT>(tile(t, 1), gb, p.dos.t, q0, qlen, p.D, p.vec, tid);
+        // one wave copies the row statistics of 64 rows at a time (rows past the last repeat it and are masked)
+        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        for (int i = wave; i < 2 * ((QT + 63) / 64); i += NT / 64) {
+          const int which = i & 1, row = (i >> 1) * 64 + lane;
+          if (row < QT)
+            __builtin_amdgcn_global_load_lds((const void*)((which ? del : lse) + min(q0 + row, qlen - 1)),
+                                             (__attribute__((address_space(3))) void*)(stats(t) + which * QT + (i >> 1) * 64), 4, 0, 0);
+        }
+      };
+      __syncthreads();   // the last head's tiles and bias are done with
+      if (SH::NBUF == 2) load(0);
+      build_ext<T>(p, h, ext0, tid, NT);
+      const float blo = table_at<T>(p, p.side - 1, h) * kLog2e, bhi = p.causal ? 0.f : table_at<T>(p, 2 * p.side - 1, h) * kLog2e;
+      for (int t = 0; t < ntile; ++t) {
+        if constexpr (SH::NBUF == 2) {
+          lds_ready();
+          if (t + 1 < ntile) load(t + 1);
+        } else {
+          __syncthreads();
+          load(t);
+          lds_ready();
+        }
+        const char *sq = tile(t, 0), *sg = tile(t, 1);
+        const float* st = stats(t);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          const int j2 = ws + WS * n, qq = qbeg + t * QT + 32 * j2, pmin = pos0 + qq, pmax = pmin + 31;
+          if (qq >= qend) break;
+          if (p.causal && pmax < wk0) continue;
+          const int dmax = wk0 + 31 - pmin, dmin = wk0 - pmax;
+          f32x16 s, dp;
+          zero16(dp);
+          float off = 0.f;
+          if (dmax <= -p.dsat) { off = blo; zero16(s); }
+          else if (!p.causal && dmin >= p.dsat) { off = bhi; zero16(s); }
+          else {
+            const float* e = ext + (ki - pmin - 4 * hh);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) s[j] = e[-acc_row(j, 0)];
+          }
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            El<T>::mma(TL::row(sq, 32 * j2 + r, 2 * ks + hh), kf[ks], s);
+            El<T>::mma(TL::row(sg, 32 * j2 + r, 2 * ks + hh), vf[ks], dp);
+          }
+          float pr[16], ds[16];
+#pragma unroll
+          for (int jg = 0; jg < 4; ++jg) {
+            const f32x4 ls = *(const f32x4*)(st + 32 * j2 + 8 * jg + 4 * hh), de = *(const f32x4*)(st + QT + 32 * j2 + 8 * jg + 4 * hh);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int j = 4 * jg + e;
+              pr[j] = expo<T>(s[j], p.c, off, ls[e]);
+              ds[j] = pr[j] * (dp[j] - de[e]);
+            }
+          }
+          if (wk0 + 31 >= klen || qq + 31 >= qlen || (p.causal && dmax > 0)) {
+            // rows that see this lane's key
+            const int first = p.causal ? ki - pmin - 4 * hh : -64, last = in ? qlen - qq - 4 * hh : -64;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const bool see = acc_row(j, 0) >= first && acc_row(j, 0) < last;
+              pr[j] = see ? pr[j] : 0.f;
+              ds[j] = see ? ds[j] : 0.f;
+            }
+          }
+#pragma unroll
+          for (int tt = 0; tt < 2; ++tt) {
+            const frag pf = El<T>::pack(pr + 8 * tt), df = El<T>::pack(ds + 8 * tt);
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+              El<T>::mma(TL::col(sg, 32 * j2 + 16 * tt, d, lane), pf, dv[d]);
+              El<T>::mma(TL::col(sq, 32 * j2 + 16 * tt, d, lane), df, dk[d]);
+            }
+          }
+        }
+      }
+    }
+  }
+  // rows behind the sequence are zeros whatever the streamed rows hold
+  const int v4 = p.D % 4 == 0;
+  const long half = (long)p.gsplit * p.B * p.Tk * p.Hkv * p.D;
+  auto part = [&](int row) { return p.gpart + ((((long)gs * p.B + b) * p.Tk + row) * p.Hkv + hk) * p.D; };
+  T* ko = (T*)p.dk + b * p.dks.b + hk * p.dks.h;
+  T* vo = (T*)p.dv + b * p.dvs.b + hk * p.dvs.h;
+  if constexpr (WS == 1) {
+    if (ki >= p.Tk) return;
+    if (p.gsplit > 1) {
+      if (in) {
+        store_rows<float, DP>(part(ki), dk, p.scale, p.D, v4, hh);
+        store_rows<float, DP>(part(ki) + half, dv, 1.f, p.D, v4, hh);
+      } else {
+        zero_rows<float, DP>(part(ki), p.D, v4, hh);
+        zero_rows<float, DP>(part(ki) + half, p.D, v4, hh);
+      }
+    } else if (in) {
+      store_rows<T, DP>(ko + (long)ki * p.dks.t, dk, p.scale, p.D, p.vec, hh);
+      store_rows<T, DP>(vo + (long)ki * p.dvs.t, dv, 1.f, p.D, p.vec, hh);
+    } else {
+      zero_rows<T, DP>(ko + (long)ki * p.dks.t, p.D, p.vec, hh);
+      zero_rows<T, DP>(vo + (long)ki * p.dvs.t, p.D, p.vec, hh);
+    }
+  } else {
+    join<DP, WS>(smem, dk, p.scale, ws, lane, tid, [&](int row, int d, float* x) {
+      if (k0 + row >= p.Tk) return;
+      if (k0 + row >= klen) x[0] = x[1] = x[2] = x[3] = 0.f;
+      if (p.gsplit > 1) store4_row(part(k0 + row), d, x, p.D, v4);
+      else store4_row(ko + (long)(k0 + row) * p.dks.t, d, x, p.D, p.vec);
+    });
+    join<DP, WS>(smem, dv, 1.f, ws, lane, tid, [&](int row, int d, float* x) {
+      if (k0 + row >= p.Tk) return;
+      if (k0 + row >= klen) x[0] = x[1] = x[2] = x[3] = 0.f;
+      if (p.gsplit > 1) store4_row(part(k0 + row) + half, d, x, p.D, v4);
+      else store4_row(vo + (long)(k0 + row) * p.dvs.t, d, x, p.D, p.vec);
+    });
+  }
+}
+
+// dk, dv from the head groups' sums, in order
+template <class T> __global__ __launch_bounds__(256) void ba_gsum_kernel(BaParams p) {
+  const long n = (long)p.B * p.Tk * p.Hkv * p.D, i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= 2 * n) return;
+  const bool second = i >= n;
+  const long e = second ? i - n : i, d = e % p.D, hk = e / p.D % p.Hkv, row = e / p.D / p.Hkv;
+  const float* x = p.gpart + (second ? p.gsplit * n : 0) + e;
+  float a = 0.f;
+  for (int g = 0; g < p.gsplit; ++g) a += x[g * n];
+  const BaStride st = second ? p.dvs : p.dks;
+  ((T*)(second ? p.dv : p.dk))[row / p.Tk * st.b + row % p.Tk * st.t + hk * st.h + d] = (T)a;
+}
+
+// ---------------------------------------------------------------- launches
+// Shared form where it gives every CU a workgroup of 128 rows, or where the spread form's LDS would not hold the table
+// sums of far borders; else the spread form. dK dV first splits the heads of a group.
+constexpr int WSP = 4;
+struct BwdPlan { bool spread_q, spread_k; int gsplit, ntq, ntk; };
+constexpr int sat_bytes(int ws) { return ws * 32 * 4 + 64; }
+BwdPlan plan_bwd(const BaParams& p) {
+  BwdPlan b;
+  const int dp = p.D <= 64 ? 64 : p.D <= 96 ? 96 : 128, spread = 8 * WSP * 32 * dp;   // the spread Shape's bytes, any type
+  b.spread_q = (long)p.B * p.Hq * ((p.Tq + 127) / 128) < 256 && spread + (1 + WSP) * host_ext_bytes(p) + sat_bytes(WSP) <= kLds;
+  b.ntq = b.spread_q ? (p.Tq + 31) / 32 : (p.Tq + 127) / 128;
+  const long keys = (long)p.B * p.Hkv * ((p.Tk + 127) / 128);
+  b.spread_k = keys * p.G < 256;
+  b.ntk = b.spread_k ? (p.Tk + 31) / 32 : (p.Tk + 127) / 128;
+  b.gsplit = (b.spread_k ? (long)p.B * p.Hkv * b.ntk < 256 : keys < 512) ? p.G : 1;
+  return b;
+}
+
+template <class T, int DP, int WR, int WS> hipError_t bwd_q(BaParams p, const BwdPlan& b, hipStream_t s) {
+  typedef Shape<T, DP, WS> SH;
+  static_assert(WS == 1 || (WS * DP * 33 * 4 <= SH::BYTES && SH::BYTES == 8 * WSP * 32 * DP), "join");
+  const long grid = (long)p.B * p.Hq * b.ntq;
+  p.ntile = b.ntq;
+  p.zigzag = grid <= 512;
+  return launch(ba_dq_kernel<T, DP, WR, WS>, grid, 64 * WR * WS, SH::BYTES + (1 + WR * WS) * host_ext_bytes(p) + sat_bytes(WS), p, s);
+}
+template <class T, int DP, int WR, int WS> hipError_t bwd_k(BaParams p, const BwdPlan& b, hipStream_t s) {
+  typedef Shape<T, DP, WS> SH;
+  const long grid = (long)p.B * p.Hkv * b.gsplit * b.ntk;
+  p.ntile = b.ntk;
+  p.zigzag = grid <= 512;
+  return launch(ba_dkv_kernel<T, DP, WR, WS>, grid, 64 * WR * WS, SH::BYTES + SH::NBUF * 2 * SH::KT * 4 + host_ext_bytes(p), p, s);
+}
+template <class T, int DP> hipError_t bwd(const BaParams& p, const BwdPlan& b, hipStream_t s) {
+  hipError_t e = b.spread_q ? bwd_q<T, DP, 1, WSP>(p, b, s) : bwd_q<T, DP, 4, 1>(p, b, s);
+  if (e == hipSuccess) e = b.spread_k ? bwd_k<T, DP, 1, WSP>(p, b, s) : bwd_k<T, DP, 4, 1>(p, b, s);
+  if (e != hipSuccess) return e;
+  if (p.gsplit > 1) {
+    const long n = 2L * p.B * p.Tk * p.Hkv * p.D, blocks = (n + 255) / 256;
+    if (blocks > 0x7fffffffL) return hipErrorInvalidValue;
+    if (blocks) hipLaunchKernelGGL((ba_gsum_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, p);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL((ba_dtable_kernel<T>), dim3((unsigned)(p.nb * p.Hq)), dim3(64), 0, s, p.tpart, (long)p.B * b.ntq,
+                     (T*)p.dtable);
+  return hipGetLastError();
+}
+template <class T> hipError_t bwd_t(const BaParams& p, const BwdPlan& b, hipStream_t s) {
+  return p.D <= 64 ? bwd<T, 64>(p, b, s) : p.D <= 96 ? bwd<T, 96>(p, b, s) : bwd<T, 128>(p, b, s);
+}
+
+size_t delta_bytes(const BaParams& p) { return up256((size_t)p.B * p.Hq * p.Tq * 4); }
+size_t table_bytes(const BaParams& p, const BwdPlan& b) { return up256((size_t)p.nb * p.Hq * p.B * b.ntq * 4); }
+
+}  // namespace
+
+size_t ba_backward_ws(const BaParams& p, int) {
+  const BwdPlan b = plan_bwd(p);
+  return delta_bytes(p) + table_bytes(p, b) + (b.gsplit > 1 ? (size_t)2 * b.gsplit * p.B * p.Tk * p.Hkv * p.D * 4 : 0) + 256;
+}
+hipError_t launch_ba_backward(BaParams p, int dtype, void* ws, hipStream_t s) {
+  const BwdPlan b = plan_bwd(p);
+  char* w = align256(ws);
+  p.delta = (float*)w;
+  p.tpart = (float*)(w + delta_bytes(p));
+  p.gpart = (float*)(w + delta_bytes(p) + table_bytes(p, b));
+  p.gsplit = b.gsplit;
+  return dtype == 0 ? bwd_t<float>(p, b, s) : dtype == 1 ? bwd_t<bf16>(p, b, s) : bwd_t<f16>(p, b, s);
+}
+
+}  // namespace gt
