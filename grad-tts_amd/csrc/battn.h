@@ -18,9 +18,9 @@ struct BaParams {
   // bucket of a distance: itself below `exact`, else exact + #{k : distance >= border[k]}; all distances >= dsat share
   // the last bucket. side = buckets of one direction (bidirectional: offsets > 0 use side .. 2 side - 1)
   int nb, side, exact, nborder, dsat;
-  int border[63];
+  int border[64];                    // the unused ones beyond any distance
   const int64_t *len, *qlen, *qstart;   // [B] or null: all of Tk, all of Tq, 0
-  int ntile, zigzag;                 // tiles of the launch's stationary side and their order (tile_of)
+  int ntile, zigzag, pair;           // tiles of the launch's stationary side and their order (tile_of, ba_fwd_kernel)
   // forward
   void* out; BaStride os;
   float* lse;                        // [B][Hq][Tq], log2 units; +inf: no visible key

@@ -4,6 +4,8 @@
 // Two kernels, each the sole writer of its rows, so that every sum has one order: dQ (with delta and the table's
 // partial sums) streams keys past 32-row query blocks, dK dV streams queries past key blocks. Scores and dP are formed
 // in both: 7 products instead of 5, against atomics or a T x T matrix in memory.
+#include <type_traits>
+
 #include "battn_core.h"
 
 namespace gt {
@@ -42,7 +44,7 @@ template <class T, int DP, int WR, int WS>
 __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 ? 1 : 2) void ba_dq_kernel(BaParams p) {
   typedef Tile<T, DP> TL;
   typedef typename El<T>::frag frag;
-  typedef Shape<T, DP, WS> SH;
+  typedef Shape<T, DP, WR, WS> SH;
   constexpr int KT = SH::KT, NB = SH::NB, KS = DP / 16, DB = DP / 32, NT = 64 * WR * WS, NW = WR * WS;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int elen = ext_len(p);
@@ -51,8 +53,8 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 ? 1 : 2) voi
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wv % WR, ws = wv / WR;
   const int r = lane & 31, hh = lane >> 5;
   float* tacc = ext0 + (1 + wv) * elen + p.dsat + EXT;   // this wave's sums of dS by offset
-  float* sat = ext0 + (1 + NW) * elen;                   // [NW][2]; [WS][32] before
-  const int nbk = p.B * p.Hkv, bk = blockIdx.x % nbk, rest = blockIdx.x / nbk, b = bk / p.Hkv, hk = bk % p.Hkv;
+  float* sat = ext0 + (1 + NW) * elen;                   // [NW][2]; [NW][32] before
+  const int nbk = p.B * p.Hkv, bk = blockIdx.x % (unsigned)nbk, rest = blockIdx.x / (unsigned)nbk, b = bk / p.Hkv, hk = bk % p.Hkv;
   const int h = hk * p.G + rest % p.G, tl = tile_of(rest / p.G, p.ntile, p.zigzag);
   const int qlen = clamp_len(p.qlen, b, p.Tq), klen = clamp_len(p.len, b, p.Tk), pos0 = start_of(p, b);
   const int q0 = tl * 32 * WR, wq0 = q0 + 32 * wr, qi = wq0 + r;
@@ -62,9 +64,12 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 ? 1 : 2) voi
   const T* kb = (const T*)p.k + b * p.ks.b + hk * p.ks.h;
   const T* vb = (const T*)p.v + b * p.vs.b + hk * p.vs.h;
   auto tile = [&](int t, int which) { return smem + ((SH::NBUF == 2 ? t & 1 : 0) * 2 + which) * SH::TILE; };
+  Stage<T, DP, KT, NT> ks, vs;
+  ks.init(kb, p.ks.t, klen, p.D, p.vec, tid);
+  vs.init(vb, p.vs.t, klen, p.D, p.vec, tid);
   auto load = [&](int t) {
-    stage<T, DP, KT, NT>(tile(t, 0), kb, p.ks.t, t * KT, klen, p.D, p.vec, tid);
-    stage<T, DP, KT, NT>(tile(t, 1), vb, p.vs.t, t * KT, klen, p.D, p.vec, tid);
+    ks.load(tile(t, 0), t * KT);
+    vs.load(tile(t, 1), t * KT);
   };
   const int ntile = kend > 0 ? (kend + KT - 1) / KT : 0;
   if (ntile && SH::NBUF == 2) load(0);
@@ -72,19 +77,15 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 ? 1 : 2) voi
   const bool in = qi < qlen;
   frag qf[KS], gf[KS];
   float delta = 0.f;
-  {
-    const T* qb = (const T*)p.q + b * p.qs.b + h * p.qs.h + (long)qi * p.qs.t;
-    const T* ob = (const T*)p.o + b * p.os.b + h * p.os.h + (long)qi * p.os.t;
-    const T* gb = (const T*)p.dout + b * p.dos.b + h * p.dos.h + (long)qi * p.dos.t;
-    f32x16 dg;
-    zero16(dg);
+  if (qlen > 0) {   // rows past the last valid one repeat it: their P is zero (lse), their results are not kept
+    const long row = min(qi, qlen - 1);
+    frag of[KS];
+    load_rows<T, KS>(qf, (const T*)p.q + b * p.qs.b + h * p.qs.h + row * p.qs.t, hh, p.D, p.vec);
+    load_rows<T, KS>(gf, (const T*)p.dout + b * p.dos.b + h * p.dos.h + row * p.dos.t, hh, p.D, p.vec);
+    load_rows<T, KS>(of, (const T*)p.o + b * p.os.b + h * p.os.h + row * p.os.t, hh, p.D, p.vec);
+    f32x16 dg = mma0<T>(of[0], gf[0]);
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      qf[s] = in ? load_row8(qb, 16 * s + 8 * hh, p.D, p.vec) : El<T>::zero();
-      gf[s] = in ? load_row8(gb, 16 * s + 8 * hh, p.D, p.vec) : El<T>::zero();
-      const frag of = in ? load_row8(ob, 16 * s + 8 * hh, p.D, p.vec) : El<T>::zero();
-      El<T>::mma(of, gf[s], dg);
-    }
+    for (int s = 1; s < KS; ++s) El<T>::mma(of[s], gf[s], dg);
     // the diagonal: row r of column r, held by lane half (r >> 2) & 1 in register (r & 3) + 4 (r >> 3)
 #pragma unroll
     for (int j = 0; j < 16; ++j) delta = acc_row(j, hh) == r ? dg[j] : delta;
@@ -97,7 +98,7 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 ? 1 : 2) voi
   if (ntile) {
     if (p.vec && p.D < DP)
       for (int i = 0; i < 2 * SH::NBUF; ++i) clear_pad<T, DP>(smem + i * SH::TILE, KT, p.D, tid, NT);
-    build_ext<T>(p, h, ext0, tid, NT);
+    build_ext<T>(p, h, 1, h, ext0, tid, NT);
   }
   const float blo = table_at<T>(p, p.side - 1, h) * kLog2e, bhi = p.causal ? 0.f : table_at<T>(p, 2 * p.side - 1, h) * kLog2e;
   f32x16 dq[DB];
@@ -112,28 +113,36 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 ? 1 : 2) voi
     const int dmax = kk + 31 - pmin, dmin = kk - pmax;
     f32x16 s;
     float off = 0.f;
-    zero16(dp);
-    if (dmax <= -p.dsat) { off = blo; zero16(s); }
-    else if (!p.causal && dmin >= p.dsat) { off = bhi; zero16(s); }
-    else {
+    frag a[KS], c[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) a[ks] = TL::row(sk, 32 * j2 + r, 2 * ks + hh);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) c[ks] = TL::row(sv, 32 * j2 + r, 2 * ks + hh);
+    if (dmax <= -p.dsat || dmin >= p.dsat) {
+      off = dmin < 0 ? blo : bhi;
+      s = mma0<T>(a[0], qf[0]);
+    } else {
       const float* e = ext + (kk + 4 * hh - pos);
 #pragma unroll
       for (int j = 0; j < 16; ++j) s[j] = e[acc_row(j, 0)];
+      El<T>::mma(a[0], qf[0], s);
     }
+    dp = mma0<T>(c[0], gf[0]);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      El<T>::mma(TL::row(sk, 32 * j2 + r, 2 * ks + hh), qf[ks], s);
-      El<T>::mma(TL::row(sv, 32 * j2 + r, 2 * ks + hh), gf[ks], dp);
+    for (int ks = 1; ks < KS; ++ks) {
+      El<T>::mma(a[ks], qf[ks], s);
+      El<T>::mma(c[ks], gf[ks], dp);
     }
 #pragma unroll
     for (int j = 0; j < 16; ++j) pr[j] = expo<T>(s[j], p.c, off, lse);
     if (kk + 31 >= klen || (p.causal && dmax > 0)) {
-      const int lim = nkey - kk - 4 * hh;
+      int lim = nkey - kk - 4 * hh;
+      in_branch(lim);
 #pragma unroll
       for (int j = 0; j < 16; ++j) pr[j] = acc_row(j, 0) < lim ? pr[j] : 0.f;
     }
   };
-  for (int t = 0; t < ntile; ++t) {
+  auto step = [&](int t, auto buf) {   // buf: t & 1, a constant at both calls
     if constexpr (SH::NBUF == 2) {
       lds_ready();
       if (t + 1 < ntile) load(t + 1);
@@ -142,7 +151,7 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 ? 1 : 2) voi
       load(t);
       lds_ready();
     }
-    const char *sk = tile(t, 0), *sv = tile(t, 1);
+    const char *sk = tile(buf, 0), *sv = tile(buf, 1);
     if (t == 0 && (WS > 1 ? kend : wend) <= KT) {
       float sum = 0.f;
 #pragma unroll
@@ -157,11 +166,11 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 ? 1 : 2) voi
       }
       sum = both_sum(sum);
       if constexpr (WS > 1) {   // all of the workgroup is here: its keys all lie in this tile
-        if (hh == 0) sat[32 * ws + r] = sum;
+        if (hh == 0) sat[32 * wv + r] = sum;
         __syncthreads();
         sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < WS; ++w) sum += sat[32 * w + r];
+        for (int w = 0; w < WS; ++w) sum += sat[32 * (wr + WR * w) + r];
       }
       if (nkey > 1) delta = sum;
     }
@@ -173,9 +182,14 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 ? 1 : 2) voi
       float ds[16];
       f32x16 dp;
       probs(sk, sv, kk, j2, ds, dp);
+      frag kc[2][DB];   // ahead of the arithmetic
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) kc[tt][d] = TL::col(sk, 32 * j2 + 16 * tt, d, lane);
 #pragma unroll
       for (int j = 0; j < 16; ++j) ds[j] *= dp[j] - delta;
-      if (dmax <= -p.dsat || (!p.causal && dmin >= p.dsat)) {
+      if (dmax <= -p.dsat || dmin >= p.dsat) {
         float a = 0.f;
 #pragma unroll
         for (int j = 0; j < 16; ++j) a += ds[j];
@@ -190,9 +204,13 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 ? 1 : 2) voi
       for (int tt = 0; tt < 2; ++tt) {
         const frag df = El<T>::pack(ds + 8 * tt);
 #pragma unroll
-        for (int d = 0; d < DB; ++d) El<T>::mma(TL::col(sk, 32 * j2 + 16 * tt, d, lane), df, dq[d]);
+        for (int d = 0; d < DB; ++d) El<T>::mma(kc[tt][d], df, dq[d]);
       }
     }
+  };
+  for (int t = 0; t < ntile; t += 2) {
+    step(t, std::integral_constant<int, 0>());
+    if (t + 1 < ntile) step(t + 1, std::integral_constant<int, 1>());
   }
   if (qi < p.Tq && hh == 0 && ws == 0) p.delta[srow] = in ? delta : 0.f;
   if constexpr (WS == 1) {
@@ -202,8 +220,8 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 ? 1 : 2) voi
       else zero_rows<T, DP>(qo, p.D, p.vec, hh);
     }
   } else {
-    join<DP, WS>(smem, dq, p.scale, ws, lane, tid, [&](int row, int d, float* x) {
-      const int i = q0 + row;
+    join<DP, WS>(smem, dq, p.scale, wr, ws, lane, [&](int row, int d, float* x) {
+      const int i = wq0 + row;
       if (i >= p.Tq) return;
       if (!(i < qlen)) x[0] = x[1] = x[2] = x[3] = 0.f;
       store4_row((T*)p.dq + b * p.dqs.b + h * p.dqs.h + (long)i * p.dqs.t, d, x, p.D, p.vec);
@@ -258,7 +276,7 @@ template <class T, int DP, int WR, int WS>
 __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 || DP > 96 ? 1 : 2) void ba_dkv_kernel(BaParams p) {
   typedef Tile<T, DP> TL;
   typedef typename El<T>::frag frag;
-  typedef Shape<T, DP, WS> SH;
+  typedef Shape<T, DP, WR, WS> SH;
   constexpr int QT = SH::KT, NB = SH::NB, KS = DP / 16, DB = DP / 32, NT = 64 * WR * WS;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   float* stat = (float*)(smem + SH::BYTES);   // [NBUF][2][QT]: lse, delta of the tile's rows
@@ -266,41 +284,41 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 || DP > 96 ?
   const float* ext = ext0 + p.dsat + EXT;
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wv % WR, ws = wv / WR;
   const int r = lane & 31, hh = lane >> 5;
-  const int nbk = p.B * p.Hkv, bk = blockIdx.x % nbk, rest = blockIdx.x / nbk, b = bk / p.Hkv, hk = bk % p.Hkv;
+  const int nbk = p.B * p.Hkv, bk = blockIdx.x % (unsigned)nbk, rest = blockIdx.x / (unsigned)nbk, b = bk / p.Hkv, hk = bk % p.Hkv;
   // the first key tiles have the most queries under a causal mask
-  const int gs = rest % p.gsplit, tl = p.ntile - 1 - tile_of(rest / p.gsplit, p.ntile, p.zigzag);
+  const int gpart = rest % p.gsplit, tl = p.ntile - 1 - tile_of(rest / p.gsplit, p.ntile, p.zigzag);
   const int k0 = tl * 32 * WR, wk0 = k0 + 32 * wr, ki = wk0 + r;
   const int qlen = clamp_len(p.qlen, b, p.Tq), klen = clamp_len(p.len, b, p.Tk), pos0 = start_of(p, b);
   const int qbeg = (p.causal ? max(0, k0 - pos0) : 0) / QT * QT;   // first tile with a query that sees key k0
   const int qend = k0 < klen ? qlen : 0;
-  const T* kb = (const T*)p.k + b * p.ks.b + hk * p.ks.h + (long)ki * p.ks.t;
-  const T* vb = (const T*)p.v + b * p.vs.b + hk * p.vs.h + (long)ki * p.vs.t;
   const bool in = ki < klen;
+  const T* kb = (const T*)p.k + b * p.ks.b + hk * p.ks.h + (long)min(ki, klen - 1) * p.ks.t;   // (rows past the last valid
+  const T* vb = (const T*)p.v + b * p.vs.b + hk * p.vs.h + (long)min(ki, klen - 1) * p.vs.t;   // one repeat it, masked)
   f32x16 dk[DB], dv[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) { zero16(dk[d]); zero16(dv[d]); }
   if (qbeg < qend) {
     frag kf[KS], vf[KS];
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      kf[s] = in ? load_row8(kb, 16 * s + 8 * hh, p.D, p.vec) : El<T>::zero();
-      vf[s] = in ? load_row8(vb, 16 * s + 8 * hh, p.D, p.vec) : El<T>::zero();
-    }
+    load_rows<T, KS>(kf, kb, hh, p.D, p.vec);
+    load_rows<T, KS>(vf, vb, hh, p.D, p.vec);
     if (p.vec && p.D < DP)
       for (int i = 0; i < 2 * SH::NBUF; ++i) clear_pad<T, DP>(smem + i * SH::TILE, QT, p.D, tid, NT);
     const int ntile = (qend - qbeg + QT - 1) / QT, hper = p.G / p.gsplit;
     for (int g = 0; g < hper; ++g) {
-      const int h = hk * p.G + gs * hper + g;
+      const int h = hk * p.G + gpart * hper + g;
       const T* qb = (const T*)p.q + b * p.qs.b + h * p.qs.h;
       const T* gb = (const T*)p.dout + b * p.dos.b + h * p.dos.h;
       const float* lse = p.lse + ((long)b * p.Hq + h) * p.Tq;
       const float* del = p.delta + ((long)b * p.Hq + h) * p.Tq;
       auto tile = [&](int t, int which) { return smem + ((SH::NBUF == 2 ? t & 1 : 0) * 2 + which) * SH::TILE; };
       auto stats = [&](int t) { return stat + (SH::NBUF == 2 ? t & 1 : 0) * 2 * QT; };
+      Stage<T, DP, QT, NT> qs, gs;
+      qs.init(qb, p.qs.t, qlen, p.D, p.vec, tid);
+      gs.init(gb, p.dos.t, qlen, p.D, p.vec, tid);
       auto load = [&](int t) {
         const int q0 = qbeg + t * QT;
-        stage<T, DP, QT, NT>(tile(t, 0), qb, p.qs.t, q0, qlen, p.D, p.vec, tid);
-        stage<T, DP, QT, NT>(tile(t, 1), gb, p.dos.t, q0, qlen, p.D, p.vec, tid);
+        qs.load(tile(t, 0), q0);
+        gs.load(tile(t, 1), q0);
         // one wave copies the row statistics of 64 rows at a time (rows past the last repeat it and are masked)
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         for (int i = wave; i < 2 * ((QT + 63) / 64); i += NT / 64) {
@@ -312,9 +330,9 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 || DP > 96 ?
       };
       __syncthreads();   // the last head's tiles and bias are done with
       if (SH::NBUF == 2) load(0);
-      build_ext<T>(p, h, ext0, tid, NT);
+      build_ext<T>(p, h, 1, h, ext0, tid, NT);
       const float blo = table_at<T>(p, p.side - 1, h) * kLog2e, bhi = p.causal ? 0.f : table_at<T>(p, 2 * p.side - 1, h) * kLog2e;
-      for (int t = 0; t < ntile; ++t) {
+      auto step = [&](int t, auto buf) {   // buf: t & 1, a constant at both calls
         if constexpr (SH::NBUF == 2) {
           lds_ready();
           if (t + 1 < ntile) load(t + 1);
@@ -323,8 +341,8 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 || DP > 96 ?
           load(t);
           lds_ready();
         }
-        const char *sq = tile(t, 0), *sg = tile(t, 1);
-        const float* st = stats(t);
+        const char *sq = tile(buf, 0), *sg = tile(buf, 1);
+        const float* st = stats(buf);
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
           const int j2 = ws + WS * n, qq = qbeg + t * QT + 32 * j2, pmin = pos0 + qq, pmax = pmin + 31;
@@ -332,19 +350,26 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 || DP > 96 ?
           if (p.causal && pmax < wk0) continue;
           const int dmax = wk0 + 31 - pmin, dmin = wk0 - pmax;
           f32x16 s, dp;
-          zero16(dp);
           float off = 0.f;
-          if (dmax <= -p.dsat) { off = blo; zero16(s); }
-          else if (!p.causal && dmin >= p.dsat) { off = bhi; zero16(s); }
-          else {
+          frag a[KS], c[KS];
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) a[ks] = TL::row(sq, 32 * j2 + r, 2 * ks + hh);
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) c[ks] = TL::row(sg, 32 * j2 + r, 2 * ks + hh);
+          if (dmax <= -p.dsat || dmin >= p.dsat) {
+            off = dmin < 0 ? blo : bhi;
+            s = mma0<T>(a[0], kf[0]);
+          } else {
             const float* e = ext + (ki - pmin - 4 * hh);
 #pragma unroll
             for (int j = 0; j < 16; ++j) s[j] = e[-acc_row(j, 0)];
+            El<T>::mma(a[0], kf[0], s);
           }
+          dp = mma0<T>(c[0], vf[0]);
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            El<T>::mma(TL::row(sq, 32 * j2 + r, 2 * ks + hh), kf[ks], s);
-            El<T>::mma(TL::row(sg, 32 * j2 + r, 2 * ks + hh), vf[ks], dp);
+          for (int ks = 1; ks < KS; ++ks) {
+            El<T>::mma(a[ks], kf[ks], s);
+            El<T>::mma(c[ks], vf[ks], dp);
           }
           float pr[16], ds[16];
 #pragma unroll
@@ -359,7 +384,9 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 || DP > 96 ?
           }
           if (wk0 + 31 >= klen || qq + 31 >= qlen || (p.causal && dmax > 0)) {
             // rows that see this lane's key
-            const int first = p.causal ? ki - pmin - 4 * hh : -64, last = in ? qlen - qq - 4 * hh : -64;
+            int first = p.causal ? ki - pmin - 4 * hh : -64, last = in ? qlen - qq - 4 * hh : -64;
+            in_branch(first);
+            in_branch(last);
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
               const bool see = acc_row(j, 0) >= first && acc_row(j, 0) < last;
@@ -369,21 +396,31 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 || DP > 96 ?
           }
 #pragma unroll
           for (int tt = 0; tt < 2; ++tt) {
+            frag gc[DB], qc[DB];
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+              gc[d] = TL::col(sg, 32 * j2 + 16 * tt, d, lane);
+              qc[d] = TL::col(sq, 32 * j2 + 16 * tt, d, lane);
+            }
             const frag pf = El<T>::pack(pr + 8 * tt), df = El<T>::pack(ds + 8 * tt);
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
-              El<T>::mma(TL::col(sg, 32 * j2 + 16 * tt, d, lane), pf, dv[d]);
-              El<T>::mma(TL::col(sq, 32 * j2 + 16 * tt, d, lane), df, dk[d]);
+              El<T>::mma(gc[d], pf, dv[d]);
+              El<T>::mma(qc[d], df, dk[d]);
             }
           }
         }
+      };
+      for (int t = 0; t < ntile; t += 2) {
+        step(t, std::integral_constant<int, 0>());
+        if (t + 1 < ntile) step(t + 1, std::integral_constant<int, 1>());
       }
     }
   }
   // rows behind the sequence are zeros whatever the streamed rows hold
   const int v4 = p.D % 4 == 0;
   const long half = (long)p.gsplit * p.B * p.Tk * p.Hkv * p.D;
-  auto part = [&](int row) { return p.gpart + ((((long)gs * p.B + b) * p.Tk + row) * p.Hkv + hk) * p.D; };
+  auto part = [&](int row) { return p.gpart + ((((long)gpart * p.B + b) * p.Tk + row) * p.Hkv + hk) * p.D; };
   T* ko = (T*)p.dk + b * p.dks.b + hk * p.dks.h;
   T* vo = (T*)p.dv + b * p.dvs.b + hk * p.dvs.h;
   if constexpr (WS == 1) {
@@ -404,17 +441,17 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 || DP > 96 ?
       zero_rows<T, DP>(vo + (long)ki * p.dvs.t, p.D, p.vec, hh);
     }
   } else {
-    join<DP, WS>(smem, dk, p.scale, ws, lane, tid, [&](int row, int d, float* x) {
-      if (k0 + row >= p.Tk) return;
-      if (k0 + row >= klen) x[0] = x[1] = x[2] = x[3] = 0.f;
-      if (p.gsplit > 1) store4_row(part(k0 + row), d, x, p.D, v4);
-      else store4_row(ko + (long)(k0 + row) * p.dks.t, d, x, p.D, p.vec);
+    join<DP, WS>(smem, dk, p.scale, wr, ws, lane, [&](int row, int d, float* x) {
+      if (wk0 + row >= p.Tk) return;
+      if (wk0 + row >= klen) x[0] = x[1] = x[2] = x[3] = 0.f;
+      if (p.gsplit > 1) store4_row(part(wk0 + row), d, x, p.D, v4);
+      else store4_row(ko + (long)(wk0 + row) * p.dks.t, d, x, p.D, p.vec);
     });
-    join<DP, WS>(smem, dv, 1.f, ws, lane, tid, [&](int row, int d, float* x) {
-      if (k0 + row >= p.Tk) return;
-      if (k0 + row >= klen) x[0] = x[1] = x[2] = x[3] = 0.f;
-      if (p.gsplit > 1) store4_row(part(k0 + row) + half, d, x, p.D, v4);
-      else store4_row(vo + (long)(k0 + row) * p.dvs.t, d, x, p.D, p.vec);
+    join<DP, WS>(smem, dv, 1.f, wr, ws, lane, [&](int row, int d, float* x) {
+      if (wk0 + row >= p.Tk) return;
+      if (wk0 + row >= klen) x[0] = x[1] = x[2] = x[3] = 0.f;
+      if (p.gsplit > 1) store4_row(part(wk0 + row) + half, d, x, p.D, v4);
+      else store4_row(vo + (long)(wk0 + row) * p.dvs.t, d, x, p.D, p.vec);
     });
   }
 }
@@ -433,41 +470,46 @@ template <class T> __global__ __launch_bounds__(256) void ba_gsum_kernel(BaParam
 }
 
 // ---------------------------------------------------------------- launches
-// Shared form where it gives every CU a workgroup of 128 rows, or where the spread form's LDS would not hold the table
-// sums of far borders; else the spread form. dK dV first splits the heads of a group.
-constexpr int WSP = 4;
-struct BwdPlan { bool spread_q, spread_k; int gsplit, ntq, ntk; };
-constexpr int sat_bytes(int ws) { return ws * 32 * 4 + 64; }
+// Rows of a workgroup: 128, or 64 where that leaves fewer than two workgroups a CU, or 32 (spread) where 64 leave every
+// other CU idle (not where the spread form's LDS would not hold the table sums of far borders). dK dV first splits the
+// heads of a group.
+constexpr int kSat = 4 * 32 * 4;   // bytes of `sat`, four waves
+struct BwdPlan { int rows_q, rows_k, gsplit, ntq, ntk; };
+int rows_of(long heads, int T) {
+  return heads * ((T + 127) / 128) >= 512 ? 128 : heads * ((T + 63) / 64) >= 128 ? 64 : 32;
+}
 BwdPlan plan_bwd(const BaParams& p) {
   BwdPlan b;
-  const int dp = p.D <= 64 ? 64 : p.D <= 96 ? 96 : 128, spread = 8 * WSP * 32 * dp;   // the spread Shape's bytes, any type
-  b.spread_q = (long)p.B * p.Hq * ((p.Tq + 127) / 128) < 256 && spread + (1 + WSP) * host_ext_bytes(p) + sat_bytes(WSP) <= kLds;
-  b.ntq = b.spread_q ? (p.Tq + 31) / 32 : (p.Tq + 127) / 128;
-  const long keys = (long)p.B * p.Hkv * ((p.Tk + 127) / 128);
-  b.spread_k = keys * p.G < 256;
-  b.ntk = b.spread_k ? (p.Tk + 31) / 32 : (p.Tk + 127) / 128;
-  b.gsplit = (b.spread_k ? (long)p.B * p.Hkv * b.ntk < 256 : keys < 512) ? p.G : 1;
+  const int dp = p.D <= 64 ? 64 : p.D <= 96 ? 96 : 128, spread = 1024 * dp;   // the spread Shape's bytes, any type
+  b.rows_q = rows_of((long)p.B * p.Hq, p.Tq);
+  if (b.rows_q == 32 && spread + 5 * host_ext_bytes(p) + kSat > kLds) b.rows_q = 64;
+  b.ntq = (p.Tq + b.rows_q - 1) / b.rows_q;
+  const long kv = (long)p.B * p.Hkv;
+  b.rows_k = rows_of(kv * p.G, p.Tk);
+  b.ntk = (p.Tk + b.rows_k - 1) / b.rows_k;
+  b.gsplit = kv * b.ntk < 512 ? p.G : 1;
   return b;
 }
 
-template <class T, int DP, int WR, int WS> hipError_t bwd_q(BaParams p, const BwdPlan& b, hipStream_t s) {
-  typedef Shape<T, DP, WS> SH;
-  static_assert(WS == 1 || (WS * DP * 33 * 4 <= SH::BYTES && SH::BYTES == 8 * WSP * 32 * DP), "join");
+template <class T, int DP, int WR> hipError_t bwd_q(BaParams p, const BwdPlan& b, hipStream_t s) {
+  typedef Shape<T, DP, WR, 4 / WR> SH;
+  static_assert(WR > 1 || SH::BYTES == 1024 * DP, "plan_bwd");
   const long grid = (long)p.B * p.Hq * b.ntq;
   p.ntile = b.ntq;
   p.zigzag = grid <= 512;
-  return launch(ba_dq_kernel<T, DP, WR, WS>, grid, 64 * WR * WS, SH::BYTES + (1 + WR * WS) * host_ext_bytes(p) + sat_bytes(WS), p, s);
+  return launch(ba_dq_kernel<T, DP, WR, 4 / WR>, grid, 256, SH::BYTES + 5 * host_ext_bytes(p) + kSat, p, s);
 }
-template <class T, int DP, int WR, int WS> hipError_t bwd_k(BaParams p, const BwdPlan& b, hipStream_t s) {
-  typedef Shape<T, DP, WS> SH;
+template <class T, int DP, int WR> hipError_t bwd_k(BaParams p, const BwdPlan& b, hipStream_t s) {
+  typedef Shape<T, DP, WR, 4 / WR> SH;
   const long grid = (long)p.B * p.Hkv * b.gsplit * b.ntk;
   p.ntile = b.ntk;
   p.zigzag = grid <= 512;
-  return launch(ba_dkv_kernel<T, DP, WR, WS>, grid, 64 * WR * WS, SH::BYTES + SH::NBUF * 2 * SH::KT * 4 + host_ext_bytes(p), p, s);
+  return launch(ba_dkv_kernel<T, DP, WR, 4 / WR>, grid, 256, SH::BYTES + SH::NBUF * 2 * SH::KT * 4 + host_ext_bytes(p), p, s);
 }
 template <class T, int DP> hipError_t bwd(const BaParams& p, const BwdPlan& b, hipStream_t s) {
-  hipError_t e = b.spread_q ? bwd_q<T, DP, 1, WSP>(p, b, s) : bwd_q<T, DP, 4, 1>(p, b, s);
-  if (e == hipSuccess) e = b.spread_k ? bwd_k<T, DP, 1, WSP>(p, b, s) : bwd_k<T, DP, 4, 1>(p, b, s);
+  hipError_t e = b.rows_q == 128 ? bwd_q<T, DP, 4>(p, b, s) : b.rows_q == 64 ? bwd_q<T, DP, 2>(p, b, s) : bwd_q<T, DP, 1>(p, b, s);
+  if (e == hipSuccess)
+    e = b.rows_k == 128 ? bwd_k<T, DP, 4>(p, b, s) : b.rows_k == 64 ? bwd_k<T, DP, 2>(p, b, s) : bwd_k<T, DP, 1>(p, b, s);
   if (e != hipSuccess) return e;
   if (p.gsplit > 1) {
     const long n = 2L * p.B * p.Tk * p.Hkv * p.D, blocks = (n + 255) / 256;

@@ -13,8 +13,9 @@
 // a 32 x 32 block lies wholly beyond the last border, as one constant: the exponent is a single FMA per score.
 //
 // A workgroup is WR row blocks x WS streams of waves: the WS waves of a row block take every WS-th 32-row block of the
-// streamed tile and join their sums through LDS at the end. WR = 4, WS = 1 shares each tile among 128 rows (long
-// sequences, where the matrix cores bound); WR = 1, WS = 4 spreads few rows over four waves (latency, memory).
+// streamed side and join their sums through LDS at the end. WR = 4, WS = 1 shares each tile among 128 rows (long
+// sequences, where the matrix cores bound), WR = 2, WS = 2 among 64 (twice the waves for as many rows), and WR = 1,
+// WS = 4 spreads few rows over four waves (latency, memory).
 #pragma once
 #include "battn.h"
 
@@ -82,6 +83,14 @@ template <> struct El<f16> {
   }
 };
 
+// a b with nothing to add to: the zero stays an inline operand instead of 16 cleared registers
+template <class T> GT_DEV f32x16 mma0(const typename El<T>::frag& a, const typename El<T>::frag& b) {
+  f32x16 c = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  El<T>::mma(a, b, c);
+  return c;
+}
+// keeps what follows inside its wave-uniform branch: the compiler would otherwise run such blocks always, with selects
+template <class X> GT_DEV void in_branch(X& x) { asm volatile("" : "+v"(x)); }
 GT_DEV void zero16(f32x16& x) {
 #pragma unroll
   for (int j = 0; j < 16; ++j) x[j] = 0.f;
@@ -94,14 +103,28 @@ GT_DEV void halves(float x, float& lo, float& hi) {   // every lane: the low and
 GT_DEV float both_sum(float x) { float a, b; halves(x, a, b); return a + b; }
 GT_DEV float both_max(float x) { float a, b; halves(x, a, b); return fmaxf(a, b); }
 
-// eight channels d .. d + 7 of one row (zero past D); `vec` as in BaParams
-template <class T> GT_DEV typename El<T>::frag load_row8(const T* p, int d, int D, int vec) {
-  if (vec) return d < D ? El<T>::load16(p + d) : El<T>::zero();
+// eight channels d .. d + 7 of one row, zero past D (rows off the 16-byte grid)
+template <class T> GT_DEV typename El<T>::frag load_row8(const T* p, int d, int D) {
   typename El<T>::frag f = El<T>::zero();
 #pragma unroll
   for (int e = 0; e < 8; ++e)
     if (d + e < D) El<T>::set(f, e, p[d + e]);
   return f;
+}
+// a row's fragments, channels 16 s + 8 h .. + 7; `vec` as in BaParams: all loads, then the cleared channels past D
+template <class T, int KS> GT_DEV void load_rows(typename El<T>::frag (&f)[KS], const T* row, int hh, int D, int vec) {
+  if (vec) {
+#pragma unroll
+    for (int s = 0; s < KS; ++s) f[s] = El<T>::load16(row + min(16 * s + 8 * hh, D - 8));
+    if (D < 16 * KS) {
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+        if (16 * s + 8 * hh >= D) f[s] = El<T>::zero();
+    }
+  } else {
+#pragma unroll
+    for (int s = 0; s < KS; ++s) f[s] = load_row8(row, 16 * s + 8 * hh, D);
+  }
 }
 
 // LDS image of a block of rows, DP channels each, as 16-byte chunks whose index is XORed, within groups of a power of
@@ -162,21 +185,28 @@ template <class T, int DP> struct Tile {
 GT_DEV int bucket_of(const BaParams& p, int delta) {   // delta = key position - query position
   const int dist = p.causal ? (delta < 0 ? -delta : 0) : (delta < 0 ? -delta : delta);
   int b = dist < p.exact ? dist : p.exact;
-  for (int k = 0; k < p.nborder; ++k) b += dist >= p.border[k];
+  for (int k = 0; k < p.nborder; k += 8)   // eight borders a scalar load; the unused ones lie beyond any distance
+#pragma unroll
+    for (int e = 0; e < 8; ++e) b += dist >= p.border[k + e];
   return b + ((!p.causal && delta > 0) ? p.side : 0);
 }
-// LDS table over the offsets -dsat - EXT .. dsat + EXT: a 32 x 32 block with an offset inside (-dsat, dsat) has all of
-// its 63 offsets in it
+// LDS table over the offsets -dsat - EXT .. dsat + EXT (causal: .. EXT): a 32 x 32 block with an offset inside
+// (-dsat, dsat) has all of its 63 offsets in it
 constexpr int EXT = 64;
-GT_DEV int ext_len(const BaParams& p) { return 2 * (p.dsat + EXT) + 1; }
+GT_DEV int ext_len(const BaParams& p) { return p.dsat + 2 * EXT + 1 + (p.causal ? 0 : p.dsat); }
 // Entries below -2^17 shut their bucket off as -inf does (rows that see only such keys are empty), entries above 2^17
 // count as 2^17: exponents stay where one FMA is exact enough
 template <class T> GT_DEV float table_at(const BaParams& p, int bucket, int h) {
   const float x = (float)((const T*)p.table)[(long)bucket * p.Hq + h];
   return x < -131072.f ? -kInf : x > 131072.f ? 131072.f : x;
 }
-template <class T> GT_DEV void build_ext(const BaParams& p, int h, float* ext, int tid, int nthreads) {
-  for (int i = tid; i < ext_len(p); i += nthreads) ext[i] = table_at<T>(p, bucket_of(p, i - p.dsat - EXT), h) * p.inv_scale;
+// bias / scale of the heads h0 .. h0 + nh - 1 (the last head again past h_last), ext_len entries each
+template <class T> GT_DEV void build_ext(const BaParams& p, int h0, int nh, int h_last, float* ext, int tid, int nthreads) {
+  const int n = ext_len(p);
+  for (int i = tid; i < n; i += nthreads) {
+    const int c = bucket_of(p, i - p.dsat - EXT);
+    for (int g = 0; g < nh; ++g) ext[g * n + i] = table_at<T>(p, c, min(h0 + g, h_last)) * p.inv_scale;
+  }
 }
 
 GT_DEV int clamp_len(const int64_t* len, int b, int most) {
@@ -200,29 +230,48 @@ GT_DEV int tile_of(int rank, int ntile, int zigzag) {
 // Aligned rows go by direct copies to LDS (16 bytes a lane; the lane's slot decides which chunk it fetches, so the image
 // comes out swizzled); rows past the last valid one repeat it, and whoever reads them masks the products. Others go
 // through registers, zero-padded. Visible after lds_ready().
-template <class T, int DP, int ROWS, int NT>
-GT_DEV void stage(char* lds, const T* base, long st, int row0, int nrow, int D, int vec, int tid) {
+template <class T, int DP, int ROWS, int NT> struct Stage {
   typedef Tile<T, DP> TL;
-  if (vec) {
-    constexpr int SLOTS = ROWS * TL::NC;
-    const int wave0 = __builtin_amdgcn_readfirstlane(tid & ~63);
+  static constexpr int SLOTS = ROWS * TL::NC, N = (SLOTS + NT - 1) / NT;
+  const T* base;
+  long st;
+  int nrow, D, vec, tid;
+  unsigned off[N];   // of this thread's chunks from the tile's first row
+  GT_DEV static int row_of(int i) { return i / TL::NC; }
+  GT_DEV static int chunk_of(int i) { return (i % TL::NC) ^ TL::swz(row_of(i)); }
+  GT_DEV void init(const T* base_, long st_, int nrow_, int D_, int vec_, int tid_) {
+    base = base_; st = st_; nrow = nrow_; D = D_; vec = vec_; tid = tid_;
 #pragma unroll
-    for (int n = 0; n < (SLOTS + NT - 1) / NT; ++n) {
-      const int i = n * NT + tid;
-      if (SLOTS % NT != 0 && i >= SLOTS) break;
-      const int row = i / TL::NC, chunk = (i % TL::NC) ^ TL::swz(row);
-      if (chunk * (16 / TL::ES) < D)
-        __builtin_amdgcn_global_load_lds((const void*)((const char*)(base + (long)min(row0 + row, nrow - 1) * st) + chunk * 16),
-                                         (__attribute__((address_space(3))) void*)(lds + (n * NT + wave0) * 16), 16, 0, 0);
-    }
-  } else {
-    constexpr int C8 = DP / 8;
-    for (int i = tid; i < ROWS * C8; i += NT) {
-      const int row = i / C8, c = i % C8;
-      TL::put(lds, row, c, row0 + row < nrow ? load_row8(base + (long)(row0 + row) * st, 8 * c, D, 0) : El<T>::zero());
+    for (int n = 0; n < N; ++n) off[n] = (unsigned)(row_of(n * NT + tid) * (int)(st * TL::ES)) + chunk_of(n * NT + tid) * 16;
+  }
+  GT_DEV void copy(char* lds, const char* from, unsigned o, int n) const {
+    __builtin_amdgcn_global_load_lds((const void*)(from + o),
+                                     (__attribute__((address_space(3))) void*)(lds + (n * NT + __builtin_amdgcn_readfirstlane(tid & ~63)) * 16), 16, 0, 0);
+  }
+  GT_DEV void load(char* lds, int row0) const {
+    if (vec) {
+      const char* from = (const char*)(base + (long)row0 * st);
+      if (D == DP && row0 + ROWS <= nrow) {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+          if (SLOTS % NT == 0 || n * NT + tid < SLOTS) copy(lds, from, off[n], n);
+      } else {
+        const int last = nrow - 1 - row0;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          const int i = n * NT + tid, over = max(row_of(i) - last, 0);
+          if ((SLOTS % NT == 0 || i < SLOTS) && chunk_of(i) * (16 / TL::ES) < D) copy(lds, from, off[n] - over * (int)(st * TL::ES), n);
+        }
+      }
+    } else {
+      constexpr int C8 = DP / 8;
+      for (int i = tid; i < ROWS * C8; i += NT) {
+        const int row = i / C8, c = i % C8;
+        TL::put(lds, row, c, row0 + row < nrow ? load_row8(base + (long)(row0 + row) * st, 8 * c, D) : El<T>::zero());
+      }
     }
   }
-}
+};
 GT_DEV void lds_ready() {   // this wave's copies have landed, then everyone's
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
@@ -268,24 +317,25 @@ template <class T> GT_DEV float expo(float acc, float c, float off, float m) {
   else return __builtin_amdgcn_exp2f(__builtin_fmaf(acc, c, off - m));
 }
 
-// Tile rows and buffers. Shared tiles (WS = 1): two buffers, the next tile's copies in flight during this one's products,
-// 16 KB a tile pair (fp32: up to 32) so that several workgroups fit a CU. Spread rows (WS > 1): 32 rows a wave;
-// 16-bit two buffers, fp32 one.
-template <class T, int DP, int WS> struct Shape {
+// Tiles shared by a workgroup: 64 streamed rows (fp32: 32 WS), two buffers, the next tile's copies in flight during this
+// one's products (fp32 with WS > 1: one, its products are long).
+constexpr int most(int a, int b) { return a > b ? a : b; }
+template <class T, int DP, int WR, int WS> struct Shape {
   static constexpr int ES = sizeof(T);
-  static constexpr int KT = WS > 1 ? 32 * WS : (ES == 2 && DP <= 64) ? 64 : 32;
-  static constexpr int NBUF = WS > 1 && ES == 4 ? 1 : 2;
+  static constexpr int KT = WS > 2 ? 32 * WS : ES == 2 ? 64 : 32 * WS;
+  static constexpr int NBUF = ES == 4 && WS > 1 ? 1 : 2;
   static constexpr int NB = KT / 32 / WS;                       // 32-row blocks of a tile for each wave
   static constexpr int TILE = KT * Tile<T, DP>::ROW;            // bytes of one operand's tile
-  static constexpr int BYTES = 2 * NBUF * TILE;
+  static constexpr int JOIN = WS > 1 ? WR * WS * DP * 33 * 4 : 0;
+  static constexpr int BYTES = most(2 * NBUF * TILE, JOIN);
 };
 
-// Sum over the WS waves of a row block, through LDS ([wave][channel][33], the tiles are done with): afterwards each
-// thread of the workgroup holds four channels of a row at a time, handed to `out(row, d, x[4])`. `mul`: this wave's
-// factor for its row (lane & 31).
+// Sum over the WS waves of a row block, through LDS ([row block][wave][channel][33], the tiles are done with): afterwards
+// each thread of the row block's waves holds four channels of a row at a time, handed to `out(row, d, x[4])`. `mul`:
+// this wave's factor for its row (lane & 31).
 template <int DP, int WS, class F>
-GT_DEV void join(char* smem, const f32x16 (&acc)[DP / 32], float mul, int ws, int lane, int tid, F out) {
-  float* s = (float*)smem;
+GT_DEV void join(char* smem, const f32x16 (&acc)[DP / 32], float mul, int wr, int ws, int lane, F out) {
+  float* s = (float*)smem + wr * (WS * DP * 33);
   const int r = lane & 31, hh = lane >> 5;
   __syncthreads();
 #pragma unroll
@@ -293,7 +343,7 @@ GT_DEV void join(char* smem, const f32x16 (&acc)[DP / 32], float mul, int ws, in
 #pragma unroll
     for (int j = 0; j < 16; ++j) s[(ws * DP + 32 * db + acc_row(j, hh)) * 33 + r] = acc[db][j] * mul;
   __syncthreads();
-  for (int i = tid; i < 32 * DP / 4; i += 64 * WS) {
+  for (int i = ws * 64 + lane; i < 32 * DP / 4; i += 64 * WS) {
     const int row = i / (DP / 4), d = i % (DP / 4) * 4;
     float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -314,7 +364,7 @@ template <class T> GT_DEV void store4_row(T* row, int d, const float* x, int D, 
 }
 
 // ---------------------------------------------------------------- launches
-inline int host_ext_bytes(const BaParams& p) { return (2 * (p.dsat + EXT) + 1) * 4; }
+inline int host_ext_bytes(const BaParams& p) { return (p.dsat + 2 * EXT + 1 + (p.causal ? 0 : p.dsat)) * 4; }
 // launches over 64 KB of LDS need the kernel's limit raised
 template <class K> hipError_t launch(K kernel, long grid, int threads, int smem, const BaParams& p, hipStream_t s) {
   if (grid > 0x7fffffffL) return hipErrorInvalidValue;

@@ -2,143 +2,58 @@
 //   o_i = sum_j softmax_j(q_i . k_j scale + table[bucket(j - pos_i)][h]) v_j ,  pos_i = q_start + i
 // T = fp32 / bf16 / fp16 operands on the matrix cores; scores, softmax statistics and sums in fp32, P rounded to T for
 // the second product (its sum l is of the unrounded terms).
+#include <type_traits>
+
 #include "battn_core.h"
 
 namespace gt {
 namespace {
 
-// One pass over the keys with the running maximum m and sum l of each row. m moves only when a row's maximum has grown
-// by 8 (in log2 units): terms stay below 2^8, and most tiles rescale nothing.
-template <class T, int DP, int WR, int WS>
-__global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 ? 1 : DP <= 64 ? 3 : 2) void ba_fwd_kernel(BaParams p) {
-  typedef Tile<T, DP> TL;
+// Running maximum and sum of a row, and its sums over v: `block` folds NB 32-key blocks in. m moves only when a row's
+// maximum has grown by 8 (in log2 units): terms stay below 2^8. The sums are rescaled by 1 all the same: behind a branch
+// the compiler copies them to other registers and back, which costs more.
+template <class T, int DP> struct Softmax {
   typedef typename El<T>::frag frag;
-  typedef Shape<T, DP, WS> SH;
-  constexpr int KT = SH::KT, NB = SH::NB, KS = DP / 16, DB = DP / 32, NT = 64 * WR * WS;
-  constexpr bool SPREAD = WS > 1;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wv % WR, ws = wv / WR;
-  const int r = lane & 31, hh = lane >> 5;
-  // ---- which rows
-  int b, hk, g0, i0, split = 0;   // first head of the group and first query
-  long blk = blockIdx.x;          // row block (spread: of all splits)
-  if constexpr (SPREAD) {
-    const int nbk = p.B * p.Hkv, ngb = (p.G + p.gp - 1) / p.gp;
-    const long units = (long)nbk * ngb * p.ntile;
-    split = (int)(blk / units);
-    blk %= units;
-    const int bk = (int)(blk % nbk), rest = (int)(blk / nbk);
-    b = bk / p.Hkv; hk = bk % p.Hkv;
-    g0 = rest % ngb * p.gp;
-    i0 = tile_of(rest / ngb, p.ntile, 0) * p.qpb;
-  } else {
-    const int nbk = p.B * p.Hkv, bk = (int)(blk % nbk), rest = (int)(blk / nbk);
-    b = bk / p.Hkv; hk = bk % p.Hkv;
-    g0 = rest % p.G;
-    i0 = tile_of(rest / p.G, p.ntile, p.zigzag) * 32 * WR;
-  }
-  const int gp = SPREAD ? p.gp : 1, rows = SPREAD ? p.qpb : 32 * WR;   // heads and queries of the workgroup
-  const int qlen = clamp_len(p.qlen, b, p.Tq), klen = clamp_len(p.len, b, p.Tk), pos0 = start_of(p, b);
-  const int wi0 = i0 + 32 * wr, wrows = SPREAD ? p.qpb : 32;           // this wave's queries
-  const int gg = SPREAD ? r % gp : 0, qi = wi0 + (SPREAD ? min(r / gp, wrows - 1) : r);
-  const int h = hk * p.G + min(g0 + gg, p.G - 1);
-  const bool mine = SPREAD ? (r < gp * wrows && g0 + gg < p.G && qi < p.Tq) : qi < p.Tq, in = mine && qi < qlen;
-  // ---- which keys
-  int kend = klen;
-  if (p.causal) kend = min(kend, pos0 + min(i0 + rows, qlen));
-  if (i0 >= qlen) kend = 0;
-  int kbeg = 0;
-  if constexpr (SPREAD) {
-    kbeg = split * p.split_keys;
-    kend = min(kend, kbeg + p.split_keys);
-  }
-  const int elen = ext_len(p);
-  float* ext0 = (float*)(smem + SH::BYTES);
-  const float* ext = ext0 + (SPREAD ? gg * elen : 0) + p.dsat + EXT;   // ext[offset]
-  const T* kb = (const T*)p.k + b * p.ks.b + hk * p.ks.h;
-  const T* vb = (const T*)p.v + b * p.vs.b + hk * p.vs.h;
-  auto tile = [&](int t, int which) { return smem + ((SH::NBUF == 2 ? t & 1 : 0) * 2 + which) * SH::TILE; };
-  auto load = [&](int t) {
-    stage<T, DP, KT, NT>(tile(t, 0), kb, p.ks.t, kbeg + t * KT, klen, p.D, p.vec, tid);
-    stage<T, DP, KT, NT>(tile(t, 1), vb, p.vs.t, kbeg + t * KT, klen, p.D, p.vec, tid);
-  };
-  const int ntile = kend > kbeg ? (kend - kbeg + KT - 1) / KT : 0;
-  if (ntile && SH::NBUF == 2) load(0);
-  frag qf[KS];
-  {
-    const T* qb = (const T*)p.q + b * p.qs.b + h * p.qs.h + (long)qi * p.qs.t;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) qf[s] = in ? load_row8(qb, 16 * s + 8 * hh, p.D, p.vec) : El<T>::zero();
-  }
-  if (ntile) {
-    if (p.vec && p.D < DP)
-      for (int i = 0; i < 2 * SH::NBUF; ++i) clear_pad<T, DP>(smem + i * SH::TILE, KT, p.D, tid, NT);
-    for (int g = 0; g < gp; ++g) build_ext<T>(p, hk * p.G + min(g0 + g, p.G - 1), ext0 + g * elen, tid, NT);
-  }
-  const float blo = table_at<T>(p, p.side - 1, h) * kLog2e, bhi = p.causal ? 0.f : table_at<T>(p, 2 * p.side - 1, h) * kLog2e;
+  static constexpr int DB = DP / 32;
   f32x16 o[DB];
+  float m, l;
+  GT_DEV void clear() {
 #pragma unroll
-  for (int d = 0; d < DB; ++d) zero16(o[d]);
-  float m = -kInf, l = 0.f;
-  const int pos = pos0 + qi, pmin = pos0 + wi0, pmax = pmin + wrows - 1;
-  const int nkey = p.causal ? min(klen, pos + 1) : klen;                       // keys this lane's row sees
-  const int wend = wi0 >= qlen ? 0 : p.causal ? min(kend, pmax + 1) : kend;    // keys this wave looks at
-  for (int t = 0; t < ntile; ++t) {
-    if constexpr (SH::NBUF == 2) {
-      lds_ready();
-      if (t + 1 < ntile) load(t + 1);
-    } else {
-      __syncthreads();
-      load(t);
-      lds_ready();
-    }
-    const int k0 = kbeg + t * KT + 32 * ws;
-    if (k0 >= wend) continue;
-    const char *sk = tile(t, 0), *sv = tile(t, 1);
-    f32x16 s[NB];
-    float off[NB], mt = -kInf;
+    for (int d = 0; d < DB; ++d) zero16(o[d]);
+    m = -kInf;
+    l = 0.f;
+  }
+  // s: scores / c (without off), -inf where unseen; col(n, tt, d): fragment of v for key group tt of block n
+  template <int NB, class Col> GT_DEV void block(const f32x16 (&s)[NB], const float (&off)[NB], float c, Col col) {
+    float mt = -kInf;
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
-      const int kk = k0 + 32 * WS * n, dmax = kk + 31 - pmin, dmin = kk - pmax;   // offsets of the block
-      off[n] = 0.f;
-      if (dmax <= -p.dsat) { off[n] = blo; zero16(s[n]); }
-      else if (!p.causal && dmin >= p.dsat) { off[n] = bhi; zero16(s[n]); }
-      else if (dmin > p.dsat) zero16(s[n]);   // causal, wholly unseen
-      else {
-        const float* e = ext + (kk + 4 * hh - pos);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) s[n][j] = e[acc_row(j, 0)];
-      }
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) El<T>::mma(TL::row(sk, 32 * (ws + WS * n) + r, 2 * ks + hh), qf[ks], s[n]);
-      if (kk + 31 >= klen || (p.causal && dmax > 0)) {
-        const int lim = nkey - kk - 4 * hh;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) s[n][j] = acc_row(j, 0) < lim ? s[n][j] : -kInf;
-      }
       float mx = fmaxf(fmaxf(s[n][0], s[n][1]), s[n][2]);
 #pragma unroll
       for (int j = 3; j < 15; j += 2) mx = fmaxf(fmaxf(s[n][j], s[n][j + 1]), mx);
-      mt = fmaxf(mt, __builtin_fmaf(fmaxf(mx, s[n][15]), p.c, off[n]));
+      mt = fmaxf(mt, __builtin_fmaf(fmaxf(mx, s[n][15]), c, off[n]));
     }
     mt = both_max(mt);
-    if (__any(mt > m + 8.f || (m == -kInf && mt > -kInf))) {
-      const float mn = fmaxf(m, mt), al = __builtin_amdgcn_exp2f(m - (mn == -kInf ? 0.f : mn));
-      m = mn;
-      l *= al;
+    const float mn = mt > m + 8.f || m == -kInf ? fmaxf(m, mt) : m, mu = mn == -kInf ? 0.f : mn;
+    const float al = __builtin_amdgcn_exp2f(m - mu);
+    m = mn;
+    l *= al;
 #pragma unroll
-      for (int d = 0; d < DB; ++d)
+    for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) o[d][j] *= al;
-    }
-    const float mu = m == -kInf ? 0.f : m;
+      for (int j = 0; j < 16; ++j) o[d][j] *= al;
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
+      frag vf[2][DB];   // read ahead of the exponentials: an LDS read waited for before every product costs more than those
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) vf[tt][d] = col(n, tt, d);
       float pr[16], sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
       for (int j = 0; j < 16; j += 2) {
-        pr[j] = expo<T>(s[n][j], p.c, off[n], mu);
-        pr[j + 1] = expo<T>(s[n][j + 1], p.c, off[n], mu);
+        pr[j] = expo<T>(s[n][j], c, off[n], mu);
+        pr[j + 1] = expo<T>(s[n][j + 1], c, off[n], mu);
         sum0 += pr[j];
         sum1 += pr[j + 1];
       }
@@ -147,55 +62,300 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 ? 1 : DP <= 
       for (int tt = 0; tt < 2; ++tt) {
         const frag pf = El<T>::pack(pr + 8 * tt);
 #pragma unroll
-        for (int d = 0; d < DB; ++d) El<T>::mma(TL::col(sv, 32 * (ws + WS * n) + 16 * tt, d, lane), pf, o[d]);
+        for (int d = 0; d < DB; ++d) El<T>::mma(vf[tt][d], pf, o[d]);
       }
     }
   }
-  l = both_sum(l);
-  const long stat = ((long)b * p.Hq + h) * p.Tq + qi;
-  if constexpr (!SPREAD) {
-    if (!mine) return;
-    T* ob = (T*)p.out + b * p.os.b + h * p.os.h + (long)qi * p.os.t;
-    const bool live = in && l != 0.f;
-    if (live) store_rows<T, DP>(ob, o, 1.f / l, p.D, p.vec, hh);
-    else zero_rows<T, DP>(ob, p.D, p.vec, hh);
-    if (p.lse && hh == 0) p.lse[stat] = live ? m + __builtin_amdgcn_logf(l) : kInf;
+};
+
+// A row's position in the sequence and what of the keys its wave looks at
+struct Seen {
+  int pos, pmin, pmax, nkey, wend;   // this lane's position, the wave's first and last; keys the lane sees, the wave visits
+  float blo, bhi;                    // bias beyond the last border, log2 units
+  const float* ext;                  // bias / scale by offset (this lane's head)
+};
+// scores / c of the 32 keys from kk on; a: their row fragments
+template <class T, int KS>
+GT_DEV void score_block(const BaParams& p, const Seen& w, int klen, int kk, int hh, const typename El<T>::frag (&a)[KS],
+                        const typename El<T>::frag (&qf)[KS], f32x16& s, float& off) {
+  const int dmax = kk + 31 - w.pmin, dmin = kk - w.pmax;   // offsets of the block
+  if (dmax <= -p.dsat || dmin >= p.dsat) {   // (causal and past the row: wholly unseen)
+    off = dmin < 0 ? w.blo : w.bhi;
+    s = mma0<T>(a[0], qf[0]);
   } else {
-    float* sml = ext0;   // [WS][2][32] (the bias table is done with)
-    __syncthreads();
-    if (hh == 0) { sml[ws * 64 + r] = m; sml[ws * 64 + 32 + r] = l; }
-    __syncthreads();
-    float M = -kInf, L = 0.f;
+    const float* e = w.ext + (kk + 4 * hh - w.pos);
+    off = 0.f;
 #pragma unroll
-    for (int w = 0; w < WS; ++w) M = fmaxf(M, sml[w * 64 + r]);
-    const float Mu = M == -kInf ? 0.f : M;
-#pragma unroll
-    for (int w = 0; w < WS; ++w) L += sml[w * 64 + 32 + r] * __builtin_amdgcn_exp2f(sml[w * 64 + r] - Mu);
-    const float f = __builtin_amdgcn_exp2f(m - Mu);
-    if (p.nsplit > 1) {
-      const long at = blk * p.nsplit + split;
-      if (tid < 32) {
-        p.part_ml[at * 64 + r] = M;
-        p.part_ml[at * 64 + 32 + r] = L;
-      }
-      if (ntile) join<DP, WS>(smem, o, f, ws, lane, tid, [&](int row, int d, const float* x) {
-        float* q = p.part + (at * 32 + row) * p.D + d;
-        if (p.D % 4 == 0) { if (d < p.D) *(f32x4*)q = (f32x4){x[0], x[1], x[2], x[3]}; }
-        else
-          for (int e = 0; e < 4; ++e) if (d + e < p.D) q[e] = x[e];
-      });
-      return;
-    }
-    const bool live = in && L != 0.f;
-    if (mine && p.lse && tid < 32) p.lse[stat] = live ? M + __builtin_amdgcn_logf(L) : kInf;
-    // the row's factor goes with the sum; dead rows come out as zeros whatever their lanes hold
-    join<DP, WS>(smem, o, live ? f / L : 0.f, ws, lane, tid, [&](int row, int d, float* x) {
-      const int g = g0 + row % gp, i = i0 + row / gp;
-      if (row >= gp * wrows || g >= p.G || i >= p.Tq) return;
-      if (!(i < qlen)) x[0] = x[1] = x[2] = x[3] = 0.f;
-      store4_row((T*)p.out + b * p.os.b + (hk * p.G + g) * p.os.h + (long)i * p.os.t, d, x, p.D, p.vec);
-    });
+    for (int j = 0; j < 16; ++j) s[j] = e[acc_row(j, 0)];
+    El<T>::mma(a[0], qf[0], s);
   }
+#pragma unroll
+  for (int ks = 1; ks < KS; ++ks) El<T>::mma(a[ks], qf[ks], s);
+  if (kk + 31 >= klen || (p.causal && dmax > 0)) {
+    int lim = w.nkey - kk - 4 * hh;
+    in_branch(lim);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) s[j] = acc_row(j, 0) < lim ? s[j] : -kInf;
+  }
+}
+template <class T> GT_DEV void far_bias(const BaParams& p, int h, Seen& w) {
+  w.blo = table_at<T>(p, p.side - 1, h) * kLog2e;
+  w.bhi = p.causal ? 0.f : table_at<T>(p, 2 * p.side - 1, h) * kLog2e;
+}
+
+// ================================================================ shared tiles
+// Under a causal mask a workgroup takes a tile from the end and its mirror image from the start (p.pair): all have the same
+// work, and none runs on alone.
+template <class T, int DP, int WR, int WS>
+__global__ __launch_bounds__(64 * WR * WS, sizeof(T) == 4 ? 1 : DP <= 64 ? 3 : 2) void ba_fwd_kernel(BaParams p) {
+  typedef Tile<T, DP> TL;
+  typedef typename El<T>::frag frag;
+  typedef Shape<T, DP, WR, WS> SH;
+  constexpr int KT = SH::KT, NB = SH::NB, KS = DP / 16, NT = 64 * WR * WS;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wv % WR, ws = wv / WR;
+  const int r = lane & 31, hh = lane >> 5;
+  const int nbk = p.B * p.Hkv, bk = blockIdx.x % (unsigned)nbk, rest = blockIdx.x / (unsigned)nbk, b = bk / p.Hkv, hk = bk % p.Hkv;
+  const int h = hk * p.G + rest % p.G, rank = rest / p.G;
+  float* ext0 = (float*)(smem + SH::BYTES);
+  build_ext<T>(p, h, 1, h, ext0, tid, NT);
+  const int qlen = clamp_len(p.qlen, b, p.Tq), klen = clamp_len(p.len, b, p.Tk), pos0 = start_of(p, b);
+  const T* kb = (const T*)p.k + b * p.ks.b + hk * p.ks.h;
+  const T* vb = (const T*)p.v + b * p.vs.b + hk * p.vs.h;
+  auto tile = [&](int t, int which) { return smem + ((SH::NBUF == 2 ? t & 1 : 0) * 2 + which) * SH::TILE; };   // LDS
+  Stage<T, DP, KT, NT> ks, vs;
+  ks.init(kb, p.ks.t, klen, p.D, p.vec, tid);
+  vs.init(vb, p.vs.t, klen, p.D, p.vec, tid);
+  auto load = [&](int t) {
+    ks.load(tile(t, 0), t * KT);
+    vs.load(tile(t, 1), t * KT);
+  };
+  if (p.vec && p.D < DP)
+    for (int i = 0; i < 2 * SH::NBUF; ++i) clear_pad<T, DP>(smem + i * SH::TILE, KT, p.D, tid, NT);
+  Seen w;
+  far_bias<T>(p, h, w);
+  w.ext = ext0 + p.dsat + EXT;
+  Softmax<T, DP> sm;
+  for (int pass = 0; pass < 2; ++pass) {
+    const int tl = pass ? rank : p.ntile - 1 - rank;
+    if (pass && (!p.pair || 2 * rank >= p.ntile - 1)) break;
+    const int i0 = tl * 32 * WR, wi0 = i0 + 32 * wr, qi = wi0 + r;
+    const bool in = qi < qlen;
+    int kend = klen;
+    if (p.causal) kend = min(kend, pos0 + min(i0 + 32 * WR, qlen));
+    if (i0 >= qlen) kend = 0;
+    const int ntile = kend > 0 ? (kend + KT - 1) / KT : 0;
+    if (pass) __syncthreads();   // the first pass's tiles are done with
+    if (ntile && SH::NBUF == 2) load(0);
+    frag qf[KS];   // (rows past the last valid one repeat it)
+    if (ntile) load_rows<T, KS>(qf, (const T*)p.q + b * p.qs.b + h * p.qs.h + (long)min(qi, qlen - 1) * p.qs.t, hh, p.D, p.vec);
+    w.pos = pos0 + qi;
+    w.pmin = pos0 + wi0;
+    w.pmax = w.pmin + 31;
+    w.nkey = p.causal ? min(klen, w.pos + 1) : klen;
+    w.wend = wi0 >= qlen ? 0 : p.causal ? min(kend, w.pmax + 1) : kend;
+    sm.clear();
+    // one tile; `buf`, a constant at both calls, is t & 1, so that LDS addresses do not depend on the loop
+    auto step = [&](int t, auto buf) {
+      if constexpr (SH::NBUF == 2) {
+        lds_ready();
+        if (t + 1 < ntile) load(t + 1);
+      } else {
+        __syncthreads();
+        load(t);
+        lds_ready();
+      }
+      const int k0 = t * KT + 32 * ws;
+      if (k0 >= w.wend) return;
+      const char *sk = tile(buf, 0), *sv = tile(buf, 1);
+      f32x16 s[NB];
+      float off[NB];
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        frag a[KS];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) a[ks] = TL::row(sk, 32 * (ws + WS * n) + r, 2 * ks + hh);
+        score_block<T, KS>(p, w, klen, k0 + 32 * WS * n, hh, a, qf, s[n], off[n]);
+      }
+      sm.template block<NB>(s, off, p.c, [&](int n, int tt, int d) { return TL::col(sv, 32 * (ws + WS * n) + 16 * tt, d, lane); });
+    };
+    for (int t = 0; t < ntile; t += 2) {
+      step(t, std::integral_constant<int, 0>());
+      if (t + 1 < ntile) step(t + 1, std::integral_constant<int, 1>());
+    }
+    const float l = both_sum(sm.l);
+    const long stat = ((long)b * p.Hq + h) * p.Tq + qi;
+    T* ob = (T*)p.out + b * p.os.b + h * p.os.h;
+    if constexpr (WS == 1) {
+      if (qi >= p.Tq) continue;
+      const bool live = in && l != 0.f;
+      if (live) store_rows<T, DP>(ob + (long)qi * p.os.t, sm.o, 1.f / l, p.D, p.vec, hh);
+      else zero_rows<T, DP>(ob + (long)qi * p.os.t, p.D, p.vec, hh);
+      if (p.lse && hh == 0) p.lse[stat] = live ? sm.m + __builtin_amdgcn_logf(l) : kInf;
+    } else {
+      float* sml = ext0 + ext_len(p) + wr * WS * 64;   // [WR][WS][2][32]
+      if (hh == 0) { sml[ws * 64 + r] = sm.m; sml[ws * 64 + 32 + r] = l; }
+      __syncthreads();
+      float M = -kInf, L = 0.f;
+#pragma unroll
+      for (int x = 0; x < WS; ++x) M = fmaxf(M, sml[x * 64 + r]);
+      const float Mu = M == -kInf ? 0.f : M;
+#pragma unroll
+      for (int x = 0; x < WS; ++x) L += sml[x * 64 + 32 + r] * __builtin_amdgcn_exp2f(sml[x * 64 + r] - Mu);
+      const bool live = in && L != 0.f;
+      if (qi < p.Tq && p.lse && hh == 0 && ws == 0) p.lse[stat] = live ? M + __builtin_amdgcn_logf(L) : kInf;
+      join<DP, WS>(smem, sm.o, live ? __builtin_amdgcn_exp2f(sm.m - Mu) / L : 0.f, wr, ws, lane, [&](int row, int d, float* x) {
+        if (wi0 + row >= p.Tq) return;
+        if (!(wi0 + row < qlen)) x[0] = x[1] = x[2] = x[3] = 0.f;
+        store4_row(ob + (long)(wi0 + row) * p.os.t, d, x, p.D, p.vec);
+      });
+    }
+  }
+}
+
+// ================================================================ spread rows
+// 32 rows -- the queries and heads that share a key / value head, packed -- and four waves, each with every fourth 32-key
+// block. No barrier in the loop. 16-bit: each wave has a slot of its own for K and one for V, refilled as soon as they are
+// read: K's copies fly during the softmax and the second product, V's during the next first one, and the LDS left over
+// holds a second workgroup. fp32: operands straight from memory (the transposed fragment's lanes are consecutive
+// channels), all of a block's loads ahead of its products.
+constexpr int WSP = 4;
+template <class T, int DP> struct Spread {
+  static constexpr bool RING = sizeof(T) == 2;
+  static constexpr int SLOT = 32 * Tile<T, DP>::ROW, WAVE = 2 * SLOT, JOIN = WSP * DP * 33 * 4;
+  static constexpr int BYTES = RING ? most(WSP * WAVE, JOIN) : JOIN;
+  static constexpr int NI = SLOT / 1024;   // copies of one slot
+};
+template <int N> GT_DEV void wait_copies() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
+GT_DEV void reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+template <class T, int DP>
+__global__ __launch_bounds__(64 * WSP, sizeof(T) == 2 || DP <= 96 ? 2 : 1) void ba_fwd_spread_kernel(BaParams p) {
+  typedef Tile<T, DP> TL;
+  typedef typename El<T>::frag frag;
+  typedef Spread<T, DP> SP;
+  constexpr int KS = DP / 16, NT = 64 * WSP;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, ws = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hh = lane >> 5;
+  const int nbk = p.B * p.Hkv, ngb = (p.G + p.gp - 1) / p.gp;
+  const unsigned units = (unsigned)nbk * ngb * p.ntile, blk = blockIdx.x % units;   // (the grid is below 2^31)
+  const int split = blockIdx.x / units;
+  const int bk = blk % (unsigned)nbk, rest = blk / (unsigned)nbk, b = bk / p.Hkv, hk = bk % p.Hkv;
+  const int g0 = rest % ngb * p.gp, i0 = tile_of(rest / ngb, p.ntile, 0) * p.qpb, gp = p.gp;
+  const int qlen = clamp_len(p.qlen, b, p.Tq), klen = clamp_len(p.len, b, p.Tk), pos0 = start_of(p, b);
+  float* ext0 = (float*)(smem + SP::BYTES);
+  build_ext<T>(p, hk * p.G + g0, gp, hk * p.G + p.G - 1, ext0, tid, NT);
+  const int gg = (unsigned)r % (unsigned)gp, qi = i0 + min((int)((unsigned)r / (unsigned)gp), p.qpb - 1), h = hk * p.G + min(g0 + gg, p.G - 1);
+  const bool mine = r < gp * p.qpb && g0 + gg < p.G && qi < p.Tq, in = mine && qi < qlen;
+  int kend = klen;
+  if (p.causal) kend = min(kend, pos0 + min(i0 + p.qpb, qlen));
+  if (i0 >= qlen) kend = 0;
+  const int kbeg = split * p.split_keys;
+  kend = min(kend, kbeg + p.split_keys);
+  const int elen = ext_len(p);
+  const T* kb = (const T*)p.k + b * p.ks.b + hk * p.ks.h;
+  const T* vb = (const T*)p.v + b * p.vs.b + hk * p.vs.h;
+  // this wave's blocks: keys kbeg + 32 (ws + 4 t)
+  const int nblk = kend > kbeg + 32 * ws ? (kend - kbeg - 32 * ws + 32 * WSP - 1) / (32 * WSP) : 0;
+  auto key0 = [&](int t) { return kbeg + 32 * (ws + WSP * t); };
+  char* mem = smem + ws * SP::WAVE;   // K, V
+  Stage<T, DP, 32, 64> ks, vs;
+  ks.init(kb, p.ks.t, klen, p.D, p.vec, lane);
+  vs.init(vb, p.vs.t, klen, p.D, p.vec, lane);
+  if (SP::RING) {
+    if (p.vec && p.D < DP)
+      for (int i = 0; i < 2; ++i) clear_pad<T, DP>(mem + i * SP::SLOT, 32, p.D, lane, 64);
+    if (nblk) {
+      ks.load(mem, key0(0));
+      vs.load(mem + SP::SLOT, key0(0));
+    }
+  }
+  frag qf[KS];
+  if (kend > kbeg) load_rows<T, KS>(qf, (const T*)p.q + b * p.qs.b + h * p.qs.h + (long)min(qi, qlen - 1) * p.qs.t, hh, p.D, p.vec);
+  Seen w;
+  far_bias<T>(p, h, w);
+  w.ext = ext0 + gg * elen + p.dsat + EXT;
+  w.pos = pos0 + qi;
+  w.pmin = pos0 + i0;
+  w.pmax = w.pmin + p.qpb - 1;
+  w.nkey = p.causal ? min(klen, w.pos + 1) : klen;
+  Softmax<T, DP> sm;
+  sm.clear();
+  lds_ready();   // the bias table (and the first blocks)
+  for (int t = 0; t < nblk; ++t) {
+    const int kk = key0(t);
+    f32x16 s[1];
+    float off[1];
+    frag a[KS];
+    if constexpr (SP::RING) {
+      const bool more = t + 1 < nblk;
+      wait_copies<SP::NI>();   // K of this block; its V may still be on its way (rows off the grid are there already)
+#pragma unroll
+      for (int x = 0; x < KS; ++x) a[x] = TL::row(mem, r, 2 * x + hh);
+      score_block<T, KS>(p, w, klen, kk, hh, a, qf, s[0], off[0]);
+      if (more) {
+        reads_done();
+        ks.load(mem, key0(t + 1));
+        wait_copies<SP::NI>();   // V of this block, K of the next behind it
+      } else {
+        wait_copies<0>();
+      }
+      sm.template block<1>(s, off, p.c, [&](int, int tt, int d) { return TL::col(mem + SP::SLOT, 16 * tt, d, lane); });
+      if (more) {
+        reads_done();
+        vs.load(mem + SP::SLOT, key0(t + 1));
+      }
+    } else {
+      frag v[2][DP / 32];
+      load_rows<T, KS>(a, kb + (long)min(kk + r, klen - 1) * p.ks.t, hh, p.D, p.vec);
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const T* vr = vb + (long)min(kk + 16 * tt + acc_row(e, hh), klen - 1) * p.vs.t;
+#pragma unroll
+          for (int d = 0; d < DP / 32; ++d)   // (channels past the head size are not stored)
+            El<T>::set(v[tt][d], e, vr[min(32 * d + r, p.D - 1)]);
+        }
+      score_block<T, KS>(p, w, klen, kk, hh, a, qf, s[0], off[0]);
+      sm.template block<1>(s, off, p.c, [&](int, int tt, int d) { return v[tt][d]; });
+    }
+  }
+  const float l = both_sum(sm.l), m = sm.m;
+  __syncthreads();     // the bias table is done with
+  float* sml = ext0;   // [WSP][2][32]
+  if (hh == 0) { sml[ws * 64 + r] = m; sml[ws * 64 + 32 + r] = l; }
+  __syncthreads();
+  float M = -kInf, L = 0.f;
+#pragma unroll
+  for (int x = 0; x < WSP; ++x) M = fmaxf(M, sml[x * 64 + r]);
+  const float Mu = M == -kInf ? 0.f : M;
+#pragma unroll
+  for (int x = 0; x < WSP; ++x) L += sml[x * 64 + 32 + r] * __builtin_amdgcn_exp2f(sml[x * 64 + r] - Mu);
+  const float f = __builtin_amdgcn_exp2f(m - Mu);
+  if (p.nsplit > 1) {
+    const long at = (long)blk * p.nsplit + split;
+    if (tid < 32) {
+      p.part_ml[at * 64 + r] = M;
+      p.part_ml[at * 64 + 32 + r] = L;
+    }
+    if (kend > kbeg) join<DP, WSP>(smem, sm.o, f, 0, ws, lane, [&](int row, int d, const float* x) {
+      float* q = p.part + (at * 32 + row) * p.D + d;
+      if (p.D % 4 == 0) { if (d < p.D) *(f32x4*)q = (f32x4){x[0], x[1], x[2], x[3]}; }
+      else
+        for (int e = 0; e < 4; ++e) if (d + e < p.D) q[e] = x[e];
+    });
+    return;
+  }
+  const bool live = in && L != 0.f;
+  if (mine && p.lse && tid < 32) p.lse[((long)b * p.Hq + h) * p.Tq + qi] = live ? M + __builtin_amdgcn_logf(L) : kInf;
+  // the row's factor goes with the sum; dead rows come out as zeros whatever their lanes hold
+  join<DP, WSP>(smem, sm.o, live ? f / L : 0.f, 0, ws, lane, [&](int row, int d, float* x) {
+    const int g = g0 + row % gp, i = i0 + row / gp;
+    if (row >= gp * p.qpb || g >= p.G || i >= p.Tq) return;
+    if (!(i < qlen)) x[0] = x[1] = x[2] = x[3] = 0.f;
+    store4_row((T*)p.out + b * p.os.b + (hk * p.G + g) * p.os.h + (long)i * p.os.t, d, x, p.D, p.vec);
+  });
 }
 
 // Joins the splits of a row: a wave a row, two channels a lane
@@ -234,20 +394,25 @@ template <class T> __global__ __launch_bounds__(256) void ba_join_kernel(BaParam
 }
 
 // ---------------------------------------------------------------- launches
-// Shared form where it fills the chip (a workgroup of 128 rows for each CU), else the spread form: rows of all heads
-// that share a key / value head packed into blocks of 32, four waves over the keys, and, where few blocks meet long
-// caches, key ranges with workgroups of their own (about four a CU, of four tiles at least) joined afterwards.
-constexpr int WSP = 4;
-struct FwdPlan { bool spread; long units; };
+// Shared tiles of 128 rows, or of 64 where that leaves fewer than two workgroups a CU, as long as these give every CU
+// one; else spread rows: blocks of 32, and, where few blocks meet long caches, key ranges with workgroups of their own
+// (about four a CU, of 512 keys at least), joined afterwards.
+enum Form { SHARED4, SHARED2, SPREAD };
+struct FwdPlan { Form form; long units; };
 FwdPlan plan_fwd(BaParams& p) {
-  const long shared = (long)p.B * p.Hq * ((p.Tq + 127) / 128);
-  FwdPlan f{shared < 256, 0};
   p.nsplit = 1;
-  if (!f.spread) {
-    p.ntile = (p.Tq + 127) / 128;
-    p.zigzag = shared <= 1024;
-    return f;
+  const long heads = (long)p.B * p.Hq;
+  auto groups = [&](int rows) {
+    p.ntile = (p.Tq + rows - 1) / rows;
+    p.pair = p.causal && p.ntile > 1;
+    return heads * (p.pair ? (p.ntile + 1) / 2 : p.ntile);
+  };
+  if (p.Tq > 32) {
+    if (groups(128) >= 512) return {SHARED4, groups(128)};
+    if (groups(64) >= 128) return {SHARED2, groups(64)};
   }
+  FwdPlan f{SPREAD, 0};
+  p.pair = 0;
   p.gp = p.G < 32 ? p.G : 32;
   while (p.gp > 1 && p.gp * host_ext_bytes(p) > 24 * 1024) p.gp = (p.gp + 1) / 2;
   p.qpb = 32 / p.gp;
@@ -255,7 +420,7 @@ FwdPlan plan_fwd(BaParams& p) {
   f.units = (long)p.B * p.Hkv * ((p.G + p.gp - 1) / p.gp) * p.ntile;
   constexpr int KT = 32 * WSP;
   p.split_keys = (p.Tk + KT - 1) / KT * KT;
-  if (f.units && f.units < 512 && p.Tk > 4 * KT) {
+  if (f.units && f.units < 256 && p.Tk > 4 * KT) {
     long n = (1024 + f.units - 1) / f.units;
     if (n > 512) n = 512;
     long keys = ((p.Tk + n - 1) / n + KT - 1) / KT * KT;
@@ -266,14 +431,18 @@ FwdPlan plan_fwd(BaParams& p) {
   return f;
 }
 
+template <class T, int DP, int WR, int WS> hipError_t shared(const BaParams& p, const FwdPlan& f, hipStream_t s) {
+  const int smem = Shape<T, DP, WR, WS>::BYTES + host_ext_bytes(p) + (WS > 1 ? WR * WS * 64 * 4 : 0);
+  return launch(ba_fwd_kernel<T, DP, WR, WS>, f.units, 64 * WR * WS, smem, p, s);
+}
 template <class T, int DP> hipError_t fwd(const BaParams& p, const FwdPlan& f, hipStream_t s) {
-  if (!f.spread)
-    return launch(ba_fwd_kernel<T, DP, 4, 1>, (long)p.B * p.Hq * p.ntile, 256, Shape<T, DP, 1>::BYTES + host_ext_bytes(p), p, s);
-  constexpr int joined = WSP * DP * 33 * 4, base = Shape<T, DP, WSP>::BYTES;
-  static_assert(joined <= base && base + 24 * 1024 <= kLds, "LDS");
+  if (f.form == SHARED4) return shared<T, DP, 4, 1>(p, f, s);
+  if (f.form == SHARED2) return shared<T, DP, 2, 2>(p, f, s);
+  constexpr int base = Spread<T, DP>::BYTES;
+  static_assert(base + 24 * 1024 <= kLds, "LDS");
   int ext = p.gp * host_ext_bytes(p);
   if (ext < WSP * 64 * 4) ext = WSP * 64 * 4;
-  hipError_t e = launch(ba_fwd_kernel<T, DP, 1, WSP>, f.units * p.nsplit, 64 * WSP, base + ext, p, s);
+  hipError_t e = launch(ba_fwd_spread_kernel<T, DP>, f.units * p.nsplit, 64 * WSP, base + ext, p, s);
   if (e != hipSuccess || p.nsplit == 1) return e;
   const long blocks = (f.units * 32 + 3) / 4;
   if (blocks > 0x7fffffffL) return hipErrorInvalidValue;

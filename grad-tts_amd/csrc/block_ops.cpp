@@ -62,14 +62,16 @@ const char* plan_buckets(int causal, int n_buckets, int max_distance, BaParams& 
   if (max_distance <= p.exact || max_distance > BA_MAX_DISTANCE)
     return "max_distance must exceed the buckets of single distances and be at most 1024";
   p.nborder = far - 1;
+  for (int& x : p.border) x = INT32_MAX;
   for (int k = 1; k < far; ++k) p.border[k - 1] = border_of(k, p.exact, far, max_distance);
   p.dsat = p.nborder ? p.border[p.nborder - 1] : p.exact;
   return nullptr;
 }
 
 BaStride st(const gt_stride& s) { return {(long)s.b, (long)s.t, (long)s.h}; }
+// rows on the 16-byte grid, 128 of them within 32-bit offsets
 bool aligned(const void* p, const gt_stride& s, int es) {
-  return ((uintptr_t)p & 15) == 0 && (s.b * es) % 16 == 0 && (s.t * es) % 16 == 0 && (s.h * es) % 16 == 0;
+  return s.t >= 0 && s.t < (1 << 21) && ((uintptr_t)p & 15) == 0 && (s.b * es) % 16 == 0 && (s.t * es) % 16 == 0 && (s.h * es) % 16 == 0;
 }
 
 constexpr int64_t kMaxT = 1 << 28;
