@@ -113,11 +113,17 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 ? 1 : 2) voi
     const int dmax = kk + 31 - pmin, dmin = kk - pmax;
     f32x16 s;
     float off = 0.f;
-    frag a[KS], c[KS];
+    // four fragments of each operand at a time: read together, then multiplied
+    constexpr int CH = KS < 4 ? KS : KS % 4 ? 3 : 4;
+    frag a[CH], c[CH];
+    auto read = [&](int k0) {
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) a[ks] = TL::row(sk, 32 * j2 + r, 2 * ks + hh);
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) c[ks] = TL::row(sv, 32 * j2 + r, 2 * ks + hh);
+      for (int x = 0; x < CH; ++x) {
+        a[x] = TL::row(sk, 32 * j2 + r, 2 * (k0 + x) + hh);
+        c[x] = TL::row(sv, 32 * j2 + r, 2 * (k0 + x) + hh);
+      }
+    };
+    read(0);
     if (dmax <= -p.dsat || dmin >= p.dsat) {
       off = dmin < 0 ? blo : bhi;
       s = mma0<T>(a[0], qf[0]);
@@ -129,9 +135,13 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 ? 1 : 2) voi
     }
     dp = mma0<T>(c[0], gf[0]);
 #pragma unroll
-    for (int ks = 1; ks < KS; ++ks) {
-      El<T>::mma(a[ks], qf[ks], s);
-      El<T>::mma(c[ks], gf[ks], dp);
+    for (int k0 = 0; k0 < KS; k0 += CH) {
+      if (k0) read(k0);
+#pragma unroll
+      for (int x = k0 ? 0 : 1; x < CH; ++x) {
+        El<T>::mma(a[x], qf[k0 + x], s);
+        El<T>::mma(c[x], gf[k0 + x], dp);
+      }
     }
 #pragma unroll
     for (int j = 0; j < 16; ++j) pr[j] = expo<T>(s[j], p.c, off, lse);
@@ -182,11 +192,9 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 ? 1 : 2) voi
       float ds[16];
       f32x16 dp;
       probs(sk, sv, kk, j2, ds, dp);
-      frag kc[2][DB];   // ahead of the arithmetic
+      frag kc[DB];   // the first group's ahead of the arithmetic
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-        for (int d = 0; d < DB; ++d) kc[tt][d] = TL::col(sk, 32 * j2 + 16 * tt, d, lane);
+      for (int d = 0; d < DB; ++d) kc[d] = TL::col(sk, 32 * j2, d, lane);
 #pragma unroll
       for (int j = 0; j < 16; ++j) ds[j] *= dp[j] - delta;
       if (dmax <= -p.dsat || dmin >= p.dsat) {
@@ -204,7 +212,10 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 ? 1 : 2) voi
       for (int tt = 0; tt < 2; ++tt) {
         const frag df = El<T>::pack(ds + 8 * tt);
 #pragma unroll
-        for (int d = 0; d < DB; ++d) El<T>::mma(kc[tt][d], df, dq[d]);
+        for (int d = 0; d < DB; ++d) {
+          El<T>::mma(kc[d], df, dq[d]);
+          if (tt == 0) kc[d] = TL::col(sk, 32 * j2 + 16, d, lane);
+        }
       }
     }
   };
@@ -470,13 +481,13 @@ template <class T> __global__ __launch_bounds__(256) void ba_gsum_kernel(BaParam
 }
 
 // ---------------------------------------------------------------- launches
-// Rows of a workgroup: 128, or 64 where that leaves fewer than two workgroups a CU, or 32 (spread) where 64 leave every
+// Rows of a workgroup: 128, or 64 where that leaves fewer than four workgroups a CU, or 32 (spread) where 64 leave every
 // other CU idle (not where the spread form's LDS would not hold the table sums of far borders). dK dV first splits the
 // heads of a group.
 constexpr int kSat = 4 * 32 * 4;   // bytes of `sat`, four waves
 struct BwdPlan { int rows_q, rows_k, gsplit, ntq, ntk; };
 int rows_of(long heads, int T) {
-  return heads * ((T + 127) / 128) >= 512 ? 128 : heads * ((T + 63) / 64) >= 128 ? 64 : 32;
+  return heads * ((T + 127) / 128) >= 1024 ? 128 : heads * ((T + 63) / 64) >= 128 ? 64 : 32;
 }
 BwdPlan plan_bwd(const BaParams& p) {
   BwdPlan b;

@@ -235,34 +235,37 @@ template <class T, int DP, int ROWS, int NT> struct Stage {
   static constexpr int SLOTS = ROWS * TL::NC, N = (SLOTS + NT - 1) / NT;
   const T* base;
   long st;
-  int nrow, D, vec, tid;
-  unsigned off[N];   // of this thread's chunks from the tile's first row
+  int nrow, D, vec, tid, wave;   // wave: LDS bytes of the wave's first lane
+  bool whole;                    // every chunk of a row is copied
+  unsigned off[N];               // of this thread's chunks from the tile's first row
   GT_DEV static int row_of(int i) { return i / TL::NC; }
   GT_DEV static int chunk_of(int i) { return (i % TL::NC) ^ TL::swz(row_of(i)); }
   GT_DEV void init(const T* base_, long st_, int nrow_, int D_, int vec_, int tid_) {
     base = base_; st = st_; nrow = nrow_; D = D_; vec = vec_; tid = tid_;
+    wave = __builtin_amdgcn_readfirstlane((tid & ~63) * 16);
+    whole = vec && D == DP;
 #pragma unroll
     for (int n = 0; n < N; ++n) off[n] = (unsigned)(row_of(n * NT + tid) * (int)(st * TL::ES)) + chunk_of(n * NT + tid) * 16;
   }
   GT_DEV void copy(char* lds, const char* from, unsigned o, int n) const {
     __builtin_amdgcn_global_load_lds((const void*)(from + o),
-                                     (__attribute__((address_space(3))) void*)(lds + (n * NT + __builtin_amdgcn_readfirstlane(tid & ~63)) * 16), 16, 0, 0);
+                                     (__attribute__((address_space(3))) void*)(lds + n * NT * 16 + wave), 16, 0, 0);
   }
   GT_DEV void load(char* lds, int row0) const {
-    if (vec) {
-      const char* from = (const char*)(base + (long)row0 * st);
-      if (D == DP && row0 + ROWS <= nrow) {
+    const char* from = (const char*)(base + (long)row0 * st);
+    if (__builtin_expect(whole && row0 + ROWS <= nrow, 1)) {
 #pragma unroll
-        for (int n = 0; n < N; ++n)
-          if (SLOTS % NT == 0 || n * NT + tid < SLOTS) copy(lds, from, off[n], n);
-      } else {
-        const int last = nrow - 1 - row0;
+      for (int n = 0; n < N; ++n)
+        if (SLOTS % NT == 0 || n * NT + tid < SLOTS) copy(lds, from, off[n], n);
+      asm volatile("; whole tile");   // (keeps the compiler from folding the two forms' copies into one behind branches)
+    } else if (vec) {
+      const int last = nrow - 1 - row0;
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-          const int i = n * NT + tid, over = max(row_of(i) - last, 0);
-          if ((SLOTS % NT == 0 || i < SLOTS) && chunk_of(i) * (16 / TL::ES) < D) copy(lds, from, off[n] - over * (int)(st * TL::ES), n);
-        }
+      for (int n = 0; n < N; ++n) {
+        const int i = n * NT + tid, over = max(row_of(i) - last, 0);
+        if ((SLOTS % NT == 0 || i < SLOTS) && chunk_of(i) * (16 / TL::ES) < D) copy(lds, from, off[n] - over * (int)(st * TL::ES), n);
       }
+      asm volatile("; part of a tile");
     } else {
       constexpr int C8 = DP / 8;
       for (int i = tid; i < ROWS * C8; i += NT) {

@@ -9,12 +9,15 @@
 namespace gt {
 namespace {
 
-// Running maximum and sum of a row, and its sums over v: `block` folds NB 32-key blocks in. m moves only when a row's
-// maximum has grown by 8 (in log2 units): terms stay below 2^8. The sums are rescaled by 1 all the same: behind a branch
-// the compiler copies them to other registers and back, which costs more.
+// Reference m and sum l of a row's exponentials 2^(score - m), and its sums over v: `block` folds NB 32-key blocks in.
+// SAFE: m is the running maximum, moved once a row's maximum has grown by 8 (in log2 units), and the sums follow it.
+// Otherwise m is the maximum of the row's first keys and stays: neither maxima nor rescaling for any later block. Terms
+// then grow up to the range of fp32 (fp16: of the type, which m starts 2^6 below), which `overflowed` sees in the sums;
+// the rows are then done again the safe way. Nothing is lost below: what lies far under the first maximum does not count.
 template <class T, int DP> struct Softmax {
   typedef typename El<T>::frag frag;
   static constexpr int DB = DP / 32;
+  static constexpr float kRoom = El<T>::wide || __is_same(T, bf16) ? 0.f : 6.f;
   f32x16 o[DB];
   float m, l;
   GT_DEV void clear() {
@@ -23,8 +26,15 @@ template <class T, int DP> struct Softmax {
     m = -kInf;
     l = 0.f;
   }
-  // s: scores / c (without off), -inf where unseen; col(n, tt, d): fragment of v for key group tt of block n
-  template <int NB, class Col> GT_DEV void block(const f32x16 (&s)[NB], const float (&off)[NB], float c, Col col) {
+  GT_DEV bool overflowed() const {
+    bool bad = !(l < kInf);
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) bad |= !(fabsf(o[d][j]) < kInf);
+    return bad;
+  }
+  template <int NB> GT_DEV static float largest(const f32x16 (&s)[NB], const float (&off)[NB], float c) {
     float mt = -kInf;
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
@@ -33,15 +43,26 @@ template <class T, int DP> struct Softmax {
       for (int j = 3; j < 15; j += 2) mx = fmaxf(fmaxf(s[n][j], s[n][j + 1]), mx);
       mt = fmaxf(mt, __builtin_fmaf(fmaxf(mx, s[n][15]), c, off[n]));
     }
-    mt = both_max(mt);
-    const float mn = mt > m + 8.f || m == -kInf ? fmaxf(m, mt) : m, mu = mn == -kInf ? 0.f : mn;
-    const float al = __builtin_amdgcn_exp2f(m - mu);
-    m = mn;
-    l *= al;
+    return both_max(mt);
+  }
+  // s: scores / c (without off), -inf where unseen; col(n, tt, d): fragment of v for key group tt of block n
+  template <bool SAFE, int NB, class Col> GT_DEV void block(const f32x16 (&s)[NB], const float (&off)[NB], float c, Col col) {
+    if constexpr (SAFE) {
+      const float mt = largest<NB>(s, off, c), mn = mt > m + 8.f || m == -kInf ? fmaxf(m, mt) : m;
+      const float al = __builtin_amdgcn_exp2f(m - (mn == -kInf ? 0.f : mn));
+      m = mn;
+      l *= al;
+      // (always: behind a branch the compiler copies the sums to other registers and back, which costs more)
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
+      for (int d = 0; d < DB; ++d)
 #pragma unroll
-      for (int j = 0; j < 16; ++j) o[d][j] *= al;
+        for (int j = 0; j < 16; ++j) o[d][j] *= al;
+    } else if (__any(m == -kInf)) {
+      float mt = largest<NB>(s, off, c) + kRoom;
+      in_branch(mt);
+      m = m == -kInf ? mt : m;
+    }
+    const float mu = m == -kInf ? 0.f : m;
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
       frag vf[2][DB];   // read ahead of the exponentials: an LDS read waited for before every product costs more than those
@@ -107,7 +128,7 @@ template <class T> GT_DEV void far_bias(const BaParams& p, int h, Seen& w) {
 // Under a causal mask a workgroup takes a tile from the end and its mirror image from the start (p.pair): all have the same
 // work, and none runs on alone.
 template <class T, int DP, int WR, int WS>
-__global__ __launch_bounds__(64 * WR * WS, sizeof(T) == 4 ? 1 : DP <= 64 ? 3 : 2) void ba_fwd_kernel(BaParams p) {
+__global__ __launch_bounds__(64 * WR * WS, sizeof(T) == 4 ? 1 : 2) void ba_fwd_kernel(BaParams p) {
   typedef Tile<T, DP> TL;
   typedef typename El<T>::frag frag;
   typedef Shape<T, DP, WR, WS> SH;
@@ -146,7 +167,6 @@ __global__ __launch_bounds__(64 * WR * WS, sizeof(T) == 4 ? 1 : DP <= 64 ? 3 : 2
     if (i0 >= qlen) kend = 0;
     const int ntile = kend > 0 ? (kend + KT - 1) / KT : 0;
     if (pass) __syncthreads();   // the first pass's tiles are done with
-    if (ntile && SH::NBUF == 2) load(0);
     frag qf[KS];   // (rows past the last valid one repeat it)
     if (ntile) load_rows<T, KS>(qf, (const T*)p.q + b * p.qs.b + h * p.qs.h + (long)min(qi, qlen - 1) * p.qs.t, hh, p.D, p.vec);
     w.pos = pos0 + qi;
@@ -154,9 +174,8 @@ __global__ __launch_bounds__(64 * WR * WS, sizeof(T) == 4 ? 1 : DP <= 64 ? 3 : 2
     w.pmax = w.pmin + 31;
     w.nkey = p.causal ? min(klen, w.pos + 1) : klen;
     w.wend = wi0 >= qlen ? 0 : p.causal ? min(kend, w.pmax + 1) : kend;
-    sm.clear();
     // one tile; `buf`, a constant at both calls, is t & 1, so that LDS addresses do not depend on the loop
-    auto step = [&](int t, auto buf) {
+    auto step = [&](int t, auto buf, auto safe) {
       if constexpr (SH::NBUF == 2) {
         lds_ready();
         if (t + 1 < ntile) load(t + 1);
@@ -177,12 +196,18 @@ __global__ __launch_bounds__(64 * WR * WS, sizeof(T) == 4 ? 1 : DP <= 64 ? 3 : 2
         for (int ks = 0; ks < KS; ++ks) a[ks] = TL::row(sk, 32 * (ws + WS * n) + r, 2 * ks + hh);
         score_block<T, KS>(p, w, klen, k0 + 32 * WS * n, hh, a, qf, s[n], off[n]);
       }
-      sm.template block<NB>(s, off, p.c, [&](int n, int tt, int d) { return TL::col(sv, 32 * (ws + WS * n) + 16 * tt, d, lane); });
+      sm.template block<decltype(safe)::value, NB>(s, off, p.c, [&](int n, int tt, int d) { return TL::col(sv, 32 * (ws + WS * n) + 16 * tt, d, lane); });
     };
-    for (int t = 0; t < ntile; t += 2) {
-      step(t, std::integral_constant<int, 0>());
-      if (t + 1 < ntile) step(t + 1, std::integral_constant<int, 1>());
-    }
+    auto run = [&](auto safe) {
+      if (ntile && SH::NBUF == 2) load(0);
+      sm.clear();
+      for (int t = 0; t < ntile; t += 2) {
+        step(t, std::integral_constant<int, 0>(), safe);
+        if (t + 1 < ntile) step(t + 1, std::integral_constant<int, 1>(), safe);
+      }
+    };
+    run(std::false_type());
+    if (__syncthreads_or(sm.overflowed())) run(std::true_type());
     const float l = both_sum(sm.l);
     const long stat = ((long)b * p.Hq + h) * p.Tq + qi;
     T* ob = (T*)p.out + b * p.os.b + h * p.os.h;
@@ -300,7 +325,7 @@ __global__ __launch_bounds__(64 * WSP, sizeof(T) == 2 || DP <= 96 ? 2 : 1) void 
       } else {
         wait_copies<0>();
       }
-      sm.template block<1>(s, off, p.c, [&](int, int tt, int d) { return TL::col(mem + SP::SLOT, 16 * tt, d, lane); });
+      sm.template block<true, 1>(s, off, p.c, [&](int, int tt, int d) { return TL::col(mem + SP::SLOT, 16 * tt, d, lane); });
       if (more) {
         reads_done();
         vs.load(mem + SP::SLOT, key0(t + 1));
@@ -318,7 +343,7 @@ __global__ __launch_bounds__(64 * WSP, sizeof(T) == 2 || DP <= 96 ? 2 : 1) void 
             El<T>::set(v[tt][d], e, vr[min(32 * d + r, p.D - 1)]);
         }
       score_block<T, KS>(p, w, klen, kk, hh, a, qf, s[0], off[0]);
-      sm.template block<1>(s, off, p.c, [&](int, int tt, int d) { return v[tt][d]; });
+      sm.template block<true, 1>(s, off, p.c, [&](int, int tt, int d) { return v[tt][d]; });
     }
   }
   const float l = both_sum(sm.l), m = sm.m;
