@@ -20,7 +20,7 @@ struct BaParams {
   int nb, side, exact, nborder, dsat;
   int border[64];                    // the unused ones beyond any distance
   const int64_t *len, *qlen, *qstart;   // [B] or null: all of Tk, all of Tq, 0
-  int ntile, zigzag, pair;           // tiles of the launch's stationary side and their order (tile_of, ba_fwd_kernel)
+  int ntile, pair;                   // tiles of the launch's stationary side; two of them a workgroup
   // forward
   void* out; BaStride os;
   float* lse;                        // [B][Hq][Tq], log2 units; +inf: no visible key
@@ -30,7 +30,7 @@ struct BaParams {
   // backward
   const void *o, *dout; BaStride dos;
   void *dq, *dk, *dv, *dtable; BaStride dqs, dks, dvs;
-  float *delta, *tpart;              // [B][Hq][Tq]; [nb][Hq][B ntile]
+  float *delta, *tpart;              // [B][Hq][Tq]; [nb][Hq][B workgroups of a head]
   int gsplit;                        // dK dV: groups of heads with workgroups of their own, summed from gpart
   float* gpart;                      // [2][gsplit][B][Tk][Hkv][D]
 };

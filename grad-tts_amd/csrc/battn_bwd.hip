@@ -41,7 +41,7 @@ GT_DEV float diagonals(const float (&x)[16]) {
 // product's gave 5.4e-3). The others take the product, from the matrix cores in the channel order of dP: so does a row
 // with one visible key (o = v), whose delta then equals dP bit for bit and whose dS is exactly zero.
 template <class T, int DP, int WR, int WS>
-__global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 ? 1 : 2) void ba_dq_kernel(BaParams p) {
+__global__ __launch_bounds__(64 * WR * WS, WS > 2 || sizeof(T) == 4 ? 1 : 2) void ba_dq_kernel(BaParams p) {
   typedef Tile<T, DP> TL;
   typedef typename El<T>::frag frag;
   typedef Shape<T, DP, WR, WS> SH;
@@ -51,16 +51,12 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 ? 1 : 2) voi
   float* ext0 = (float*)(smem + SH::BYTES);
   const float* ext = ext0 + p.dsat + EXT;
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wv % WR, ws = wv / WR;
-  const int r = lane & 31, hh = lane >> 5;
+  const int r = lane & 31, hh = lane >> 5, D = p.D;
   float* tacc = ext0 + (1 + wv) * elen + p.dsat + EXT;   // this wave's sums of dS by offset
   float* sat = ext0 + (1 + NW) * elen;                   // [NW][2]; [NW][32] before
   const int nbk = p.B * p.Hkv, bk = blockIdx.x % (unsigned)nbk, rest = blockIdx.x / (unsigned)nbk, b = bk / p.Hkv, hk = bk % p.Hkv;
-  const int h = hk * p.G + rest % p.G, tl = tile_of(rest / p.G, p.ntile, p.zigzag);
+  const int h = hk * p.G + rest % p.G, rank = rest / p.G;
   const int qlen = clamp_len(p.qlen, b, p.Tq), klen = clamp_len(p.len, b, p.Tk), pos0 = start_of(p, b);
-  const int q0 = tl * 32 * WR, wq0 = q0 + 32 * wr, qi = wq0 + r;
-  int kend = klen;
-  if (p.causal) kend = min(kend, pos0 + min(q0 + 32 * WR, qlen));
-  if (q0 >= qlen) kend = 0;
   const T* kb = (const T*)p.k + b * p.ks.b + hk * p.ks.h;
   const T* vb = (const T*)p.v + b * p.vs.b + hk * p.vs.h;
   auto tile = [&](int t, int which) { return smem + ((SH::NBUF == 2 ? t & 1 : 0) * 2 + which) * SH::TILE; };
@@ -71,6 +67,14 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 ? 1 : 2) voi
     ks.load(tile(t, 0), t * KT);
     vs.load(tile(t, 1), t * KT);
   };
+  float slo = 0.f, shi = 0.f;   // dS beyond the last border
+  const int tl = p.ntile - 1 - rank;   // the longest under a causal mask first
+  const int q0 = tl * 32 * WR, wq0 = q0 + 32 * wr, qi = wq0 + r;
+  int kend = klen;
+  if (p.causal) kend = min(kend, pos0 + min(q0 + 32 * WR, qlen));
+  if (q0 >= qlen) kend = 0;
+  if (p.vec && D < DP)
+    for (int i = 0; i < 2 * SH::NBUF; ++i) clear_pad<T, DP>(smem + i * SH::TILE, KT, D, tid, NT);
   const int ntile = kend > 0 ? (kend + KT - 1) / KT : 0;
   if (ntile && SH::NBUF == 2) load(0);
   const long srow = ((long)b * p.Hq + h) * p.Tq + qi;
@@ -80,9 +84,9 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 ? 1 : 2) voi
   if (qlen > 0) {   // rows past the last valid one repeat it: their P is zero (lse), their results are not kept
     const long row = min(qi, qlen - 1);
     frag of[KS];
-    load_rows<T, KS>(qf, (const T*)p.q + b * p.qs.b + h * p.qs.h + row * p.qs.t, hh, p.D, p.vec);
-    load_rows<T, KS>(gf, (const T*)p.dout + b * p.dos.b + h * p.dos.h + row * p.dos.t, hh, p.D, p.vec);
-    load_rows<T, KS>(of, (const T*)p.o + b * p.os.b + h * p.os.h + row * p.os.t, hh, p.D, p.vec);
+    load_rows<T, KS>(qf, (const T*)p.q + b * p.qs.b + h * p.qs.h + row * p.qs.t, hh, D, p.vec);
+    load_rows<T, KS>(gf, (const T*)p.dout + b * p.dos.b + h * p.dos.h + row * p.dos.t, hh, D, p.vec);
+    load_rows<T, KS>(of, (const T*)p.o + b * p.os.b + h * p.os.h + row * p.os.t, hh, D, p.vec);
     f32x16 dg = mma0<T>(of[0], gf[0]);
 #pragma unroll
     for (int s = 1; s < KS; ++s) El<T>::mma(of[s], gf[s], dg);
@@ -95,16 +99,11 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 ? 1 : 2) voi
   }
   const float lse = in ? p.lse[srow] : kInf;
   for (int i = tid; i < NW * elen; i += NT) ext0[elen + i] = 0.f;
-  if (ntile) {
-    if (p.vec && p.D < DP)
-      for (int i = 0; i < 2 * SH::NBUF; ++i) clear_pad<T, DP>(smem + i * SH::TILE, KT, p.D, tid, NT);
-    build_ext<T>(p, h, 1, h, ext0, tid, NT);
-  }
+  build_ext<T>(p, h, 1, h, ext0, tid, NT);
   const float blo = table_at<T>(p, p.side - 1, h) * kLog2e, bhi = p.causal ? 0.f : table_at<T>(p, 2 * p.side - 1, h) * kLog2e;
   f32x16 dq[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) zero16(dq[d]);
-  float slo = 0.f, shi = 0.f;   // dS beyond the last border
   const int pos = pos0 + qi, pmin = pos0 + wq0, pmax = pmin + 31;
   const int nkey = p.causal ? min(klen, pos + 1) : klen;                       // keys this lane's row sees
   const int wend = wq0 >= qlen ? 0 : p.causal ? min(kend, pmax + 1) : kend;    // keys this wave looks at
@@ -114,7 +113,7 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 ? 1 : 2) voi
     f32x16 s;
     float off = 0.f;
     // four fragments of each operand at a time: read together, then multiplied
-    constexpr int CH = KS < 4 ? KS : KS % 4 ? 3 : 4;
+    constexpr int CH = KS % 4 ? 3 : 4;
     frag a[CH], c[CH];
     auto read = [&](int k0) {
 #pragma unroll
@@ -227,18 +226,18 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 ? 1 : 2) voi
   if constexpr (WS == 1) {
     if (qi < p.Tq) {
       T* qo = (T*)p.dq + b * p.dqs.b + h * p.dqs.h + (long)qi * p.dqs.t;
-      if (in) store_rows<T, DP>(qo, dq, p.scale, p.D, p.vec, hh);
-      else zero_rows<T, DP>(qo, p.D, p.vec, hh);
+      if (in) store_rows<T, DP>(qo, dq, p.scale, D, p.vec, hh);
+      else zero_rows<T, DP>(qo, D, p.vec, hh);
     }
   } else {
     join<DP, WS>(smem, dq, p.scale, wr, ws, lane, [&](int row, int d, float* x) {
       const int i = wq0 + row;
       if (i >= p.Tq) return;
       if (!(i < qlen)) x[0] = x[1] = x[2] = x[3] = 0.f;
-      store4_row((T*)p.dq + b * p.dqs.b + h * p.dqs.h + (long)i * p.dqs.t, d, x, p.D, p.vec);
+      store4_row((T*)p.dq + b * p.dqs.b + h * p.dqs.h + (long)i * p.dqs.t, d, x, D, p.vec);
     });
   }
-  // table partials of this tile: a wave a bucket, its lanes over the bucket's offsets, then across the lanes in one order
+  // table partials of the workgroup: a wave a bucket, its lanes over the bucket's offsets, then across the lanes in one order
 #pragma unroll
   for (int x = 32; x > 0; x >>= 1) {
     slo += __shfl_xor(slo, x);
@@ -267,7 +266,7 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 ? 1 : 2) voi
     for (int x = 32; x > 0; x >>= 1) a += __shfl_xor(a, x);
     if (cc == p.side - 1)
       for (int w = 0; w < NW; ++w) a += sat[2 * w + side];
-    if (lane == 0) p.tpart[((long)c * p.Hq + h) * npart + (long)b * p.ntile + tl] = a;
+    if (lane == 0) p.tpart[((long)c * p.Hq + h) * npart + (long)b * p.ntile + rank] = a;
   }
 }
 
@@ -284,7 +283,7 @@ template <class T> __global__ __launch_bounds__(64) void ba_dtable_kernel(const 
 // 32 WR keys of one key / value head over the query tiles of the heads that share it, or, where that leaves CUs idle, of
 // a part of them (gsplit), summed afterwards in fp32.
 template <class T, int DP, int WR, int WS>
-__global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 || DP > 96 ? 1 : 2) void ba_dkv_kernel(BaParams p) {
+__global__ __launch_bounds__(64 * WR * WS, WS > 2 || sizeof(T) == 4 || DP > 64 ? 1 : 2) void ba_dkv_kernel(BaParams p) {
   typedef Tile<T, DP> TL;
   typedef typename El<T>::frag frag;
   typedef Shape<T, DP, WR, WS> SH;
@@ -293,212 +292,245 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 1 || sizeof(T) == 4 || DP > 96 ?
   float* stat = (float*)(smem + SH::BYTES);   // [NBUF][2][QT]: lse, delta of the tile's rows
   float* ext0 = stat + SH::NBUF * 2 * QT;
   const float* ext = ext0 + p.dsat + EXT;
-  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wv % WR, ws = wv / WR;
-  const int r = lane & 31, hh = lane >> 5;
+  const int tid = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wv % WR, ws = wv / WR;
   const int nbk = p.B * p.Hkv, bk = blockIdx.x % (unsigned)nbk, rest = blockIdx.x / (unsigned)nbk, b = bk / p.Hkv, hk = bk % p.Hkv;
-  // the first key tiles have the most queries under a causal mask
-  const int gpart = rest % p.gsplit, tl = p.ntile - 1 - tile_of(rest / p.gsplit, p.ntile, p.zigzag);
-  const int k0 = tl * 32 * WR, wk0 = k0 + 32 * wr, ki = wk0 + r;
+  const int gpart = rest % p.gsplit, rank = rest / p.gsplit;
   const int qlen = clamp_len(p.qlen, b, p.Tq), klen = clamp_len(p.len, b, p.Tk), pos0 = start_of(p, b);
-  const int qbeg = (p.causal ? max(0, k0 - pos0) : 0) / QT * QT;   // first tile with a query that sees key k0
-  const int qend = k0 < klen ? qlen : 0;
-  const bool in = ki < klen;
-  const T* kb = (const T*)p.k + b * p.ks.b + hk * p.ks.h + (long)min(ki, klen - 1) * p.ks.t;   // (rows past the last valid
-  const T* vb = (const T*)p.v + b * p.vs.b + hk * p.vs.h + (long)min(ki, klen - 1) * p.vs.t;   // one repeat it, masked)
-  f32x16 dk[DB], dv[DB];
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {   // a tile from the start and, paired, its mirror image
+    if (pass && (!p.pair || 2 * rank >= p.ntile - 1)) break;
+    const int lane = anew_v(tid & 63), r = lane & 31, hh = lane >> 5, D = anew_s(p.D);
+    const int tl = pass ? p.ntile - 1 - rank : rank;
+    const int k0 = tl * 32 * WR, wk0 = k0 + 32 * wr, ki = wk0 + r;
+    if (pass) __syncthreads();   // the first pass's LDS is done with
+    const int qbeg = (p.causal ? max(0, k0 - pos0) : 0) / QT * QT;   // first tile with a query that sees key k0
+    const int qend = k0 < klen ? qlen : 0;
+    const bool in = ki < klen;
+    const T* kb = (const T*)p.k + b * p.ks.b + hk * p.ks.h + (long)min(ki, klen - 1) * p.ks.t;   // (rows past the last valid
+    const T* vb = (const T*)p.v + b * p.vs.b + hk * p.vs.h + (long)min(ki, klen - 1) * p.vs.t;   // one repeat it, masked)
+    f32x16 dk[DB], dv[DB];
 #pragma unroll
-  for (int d = 0; d < DB; ++d) { zero16(dk[d]); zero16(dv[d]); }
-  if (qbeg < qend) {
-    frag kf[KS], vf[KS];
-    load_rows<T, KS>(kf, kb, hh, p.D, p.vec);
-    load_rows<T, KS>(vf, vb, hh, p.D, p.vec);
-    if (p.vec && p.D < DP)
-      for (int i = 0; i < 2 * SH::NBUF; ++i) clear_pad<T, DP>(smem + i * SH::TILE, QT, p.D, tid, NT);
-    const int ntile = (qend - qbeg + QT - 1) / QT, hper = p.G / p.gsplit;
-    for (int g = 0; g < hper; ++g) {
-      const int h = hk * p.G + gpart * hper + g;
-      const T* qb = (const T*)p.q + b * p.qs.b + h * p.qs.h;
-      const T* gb = (const T*)p.dout + b * p.dos.b + h * p.dos.h;
-      const float* lse = p.lse + ((long)b * p.Hq + h) * p.Tq;
-      const float* del = p.delta + ((long)b * p.Hq + h) * p.Tq;
-      auto tile = [&](int t, int which) { return smem + ((SH::NBUF == 2 ? t & 1 : 0) * 2 + which) * SH::TILE; };
-      auto stats = [&](int t) { return stat + (SH::NBUF == 2 ? t & 1 : 0) * 2 * QT; };
-      Stage<T, DP, QT, NT> qs, gs;
-      qs.init(qb, p.qs.t, qlen, p.D, p.vec, tid);
-      gs.init(gb, p.dos.t, qlen, p.D, p.vec, tid);
-      auto load = [&](int t) {
-        const int q0 = qbeg + t * QT;
-        qs.load(tile(t, 0), q0);
-        gs.load(tile(t, 1), q0);
-        // one wave copies the row statistics of 64 rows at a time (rows past the last repeat it and are masked)
-        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-        for (int i = wave; i < 2 * ((QT + 63) / 64); i += NT / 64) {
-          const int which = i & 1, row = (i >> 1) * 64 + lane;
-          if (row < QT)
-            __builtin_amdgcn_global_load_lds((const void*)((which ? del : lse) + min(q0 + row, qlen - 1)),
-                                             (__attribute__((address_space(3))) void*)(stats(t) + which * QT + (i >> 1) * 64), 4, 0, 0);
-        }
-      };
-      __syncthreads();   // the last head's tiles and bias are done with
-      if (SH::NBUF == 2) load(0);
-      build_ext<T>(p, h, 1, h, ext0, tid, NT);
-      const float blo = table_at<T>(p, p.side - 1, h) * kLog2e, bhi = p.causal ? 0.f : table_at<T>(p, 2 * p.side - 1, h) * kLog2e;
-      auto step = [&](int t, auto buf) {   // buf: t & 1, a constant at both calls
-        if constexpr (SH::NBUF == 2) {
-          lds_ready();
-          if (t + 1 < ntile) load(t + 1);
-        } else {
-          __syncthreads();
-          load(t);
-          lds_ready();
-        }
-        const char *sq = tile(buf, 0), *sg = tile(buf, 1);
-        const float* st = stats(buf);
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          const int j2 = ws + WS * n, qq = qbeg + t * QT + 32 * j2, pmin = pos0 + qq, pmax = pmin + 31;
-          if (qq >= qend) break;
-          if (p.causal && pmax < wk0) continue;
-          const int dmax = wk0 + 31 - pmin, dmin = wk0 - pmax;
-          f32x16 s, dp;
-          float off = 0.f;
-          frag a[KS], c[KS];
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks) a[ks] = TL::row(sq, 32 * j2 + r, 2 * ks + hh);
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks) c[ks] = TL::row(sg, 32 * j2 + r, 2 * ks + hh);
-          if (dmax <= -p.dsat || dmin >= p.dsat) {
-            off = dmin < 0 ? blo : bhi;
-            s = mma0<T>(a[0], kf[0]);
+    for (int d = 0; d < DB; ++d) { zero16(dk[d]); zero16(dv[d]); }
+    if (qbeg < qend) {
+      frag kf[KS], vf[KS];
+      load_rows<T, KS>(kf, kb, hh, D, p.vec);
+      load_rows<T, KS>(vf, vb, hh, D, p.vec);
+      if (p.vec && D < DP)
+        for (int i = 0; i < 2 * SH::NBUF; ++i) clear_pad<T, DP>(smem + i * SH::TILE, QT, D, tid, NT);
+      const int ntile = (qend - qbeg + QT - 1) / QT, hper = p.G / p.gsplit;
+      for (int g = 0; g < hper; ++g) {
+        const int h = hk * p.G + gpart * hper + g;
+        const T* qb = (const T*)p.q + b * p.qs.b + h * p.qs.h;
+        const T* gb = (const T*)p.dout + b * p.dos.b + h * p.dos.h;
+        const float* lse = p.lse + ((long)b * p.Hq + h) * p.Tq;
+        const float* del = p.delta + ((long)b * p.Hq + h) * p.Tq;
+        auto tile = [&](int t, int which) { return smem + ((SH::NBUF == 2 ? t & 1 : 0) * 2 + which) * SH::TILE; };
+        auto stats = [&](int t) { return stat + (SH::NBUF == 2 ? t & 1 : 0) * 2 * QT; };
+        Stage<T, DP, QT, NT> qs, gs;
+        qs.init(qb, p.qs.t, qlen, D, p.vec, tid);
+        gs.init(gb, p.dos.t, qlen, D, p.vec, tid);
+        auto load = [&](int t) {
+          const int q0 = qbeg + t * QT;
+          qs.load(tile(t, 0), q0);
+          gs.load(tile(t, 1), q0);
+          // one wave copies the row statistics of 64 rows at a time (rows past the last repeat it and are masked)
+          const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+          for (int i = wave; i < 2 * ((QT + 63) / 64); i += NT / 64) {
+            const int which = i & 1, row = (i >> 1) * 64 + lane;
+            if (row < QT)
+              __builtin_amdgcn_global_load_lds((const void*)((which ? del : lse) + min(q0 + row, qlen - 1)),
+                                               (__attribute__((address_space(3))) void*)(stats(t) + which * QT + (i >> 1) * 64), 4, 0, 0);
+          }
+        };
+        __syncthreads();   // the last head's tiles and bias are done with
+        if (SH::NBUF == 2) load(0);
+        build_ext<T>(p, h, 1, h, ext0, tid, NT);
+        const float blo = table_at<T>(p, p.side - 1, h) * kLog2e, bhi = p.causal ? 0.f : table_at<T>(p, 2 * p.side - 1, h) * kLog2e;
+        auto step = [&](int t, auto buf) {   // buf: t & 1, a constant at both calls
+          if constexpr (SH::NBUF == 2) {
+            lds_ready();
+            if (t + 1 < ntile) load(t + 1);
           } else {
-            const float* e = ext + (ki - pmin - 4 * hh);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) s[j] = e[-acc_row(j, 0)];
-            El<T>::mma(a[0], kf[0], s);
+            __syncthreads();
+            load(t);
+            lds_ready();
           }
-          dp = mma0<T>(c[0], vf[0]);
+          const char *sq = tile(buf, 0), *sg = tile(buf, 1);
+          const float* st = stats(buf);
 #pragma unroll
-          for (int ks = 1; ks < KS; ++ks) {
-            El<T>::mma(a[ks], kf[ks], s);
-            El<T>::mma(c[ks], vf[ks], dp);
-          }
-          float pr[16], ds[16];
+          for (int n = 0; n < NB; ++n) {
+            const int j2 = ws + WS * n, qq = qbeg + t * QT + 32 * j2, pmin = pos0 + qq, pmax = pmin + 31;
+            if (qq >= qend) break;
+            if (p.causal && pmax < wk0) continue;
+            const int dmax = wk0 + 31 - pmin, dmin = wk0 - pmax;
+            f32x16 s, dp;
+            float off = 0.f;
+            constexpr int CH = KS % 4 ? 3 : 4;
+            frag a[CH], c[CH];
+            auto read = [&](int x0) {
 #pragma unroll
-          for (int jg = 0; jg < 4; ++jg) {
-            const f32x4 ls = *(const f32x4*)(st + 32 * j2 + 8 * jg + 4 * hh), de = *(const f32x4*)(st + QT + 32 * j2 + 8 * jg + 4 * hh);
+              for (int x = 0; x < CH; ++x) {
+                a[x] = TL::row(sq, 32 * j2 + r, 2 * (x0 + x) + hh);
+                c[x] = TL::row(sg, 32 * j2 + r, 2 * (x0 + x) + hh);
+              }
+            };
+            read(0);
+            if (dmax <= -p.dsat || dmin >= p.dsat) {
+              off = dmin < 0 ? blo : bhi;
+              s = mma0<T>(a[0], kf[0]);
+            } else {
+              const float* e = ext + (ki - pmin - 4 * hh);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int j = 4 * jg + e;
-              pr[j] = expo<T>(s[j], p.c, off, ls[e]);
-              ds[j] = pr[j] * (dp[j] - de[e]);
+              for (int j = 0; j < 16; ++j) s[j] = e[-acc_row(j, 0)];
+              El<T>::mma(a[0], kf[0], s);
+            }
+            dp = mma0<T>(c[0], vf[0]);
+#pragma unroll
+            for (int x0 = 0; x0 < KS; x0 += CH) {
+              if (x0) read(x0);
+#pragma unroll
+              for (int x = x0 ? 0 : 1; x < CH; ++x) {
+                El<T>::mma(a[x], kf[x0 + x], s);
+                El<T>::mma(c[x], vf[x0 + x], dp);
+              }
+            }
+            float pr[16], ds[16];
+#pragma unroll
+            for (int jg = 0; jg < 4; ++jg) {
+              const f32x4 ls = *(const f32x4*)(st + 32 * j2 + 8 * jg + 4 * hh), de = *(const f32x4*)(st + QT + 32 * j2 + 8 * jg + 4 * hh);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int j = 4 * jg + e;
+                pr[j] = expo<T>(s[j], p.c, off, ls[e]);
+                ds[j] = pr[j] * (dp[j] - de[e]);
+              }
+            }
+            if (wk0 + 31 >= klen || qq + 31 >= qlen || (p.causal && dmax > 0)) {
+              // rows that see this lane's key
+              int first = p.causal ? ki - pmin - 4 * hh : -64, last = in ? qlen - qq - 4 * hh : -64;
+              in_branch(first);
+              in_branch(last);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                const bool see = acc_row(j, 0) >= first && acc_row(j, 0) < last;
+                pr[j] = see ? pr[j] : 0.f;
+                ds[j] = see ? ds[j] : 0.f;
+              }
+            }
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt) {
+              frag x[DB];
+#pragma unroll
+              for (int d = 0; d < DB; ++d) x[d] = TL::col(sg, 32 * j2 + 16 * tt, d, lane);
+              const frag pf = El<T>::pack(pr + 8 * tt), df = El<T>::pack(ds + 8 * tt);
+#pragma unroll
+              for (int d = 0; d < DB; ++d) {
+                El<T>::mma(x[d], pf, dv[d]);
+                x[d] = TL::col(sq, 32 * j2 + 16 * tt, d, lane);
+              }
+#pragma unroll
+              for (int d = 0; d < DB; ++d) El<T>::mma(x[d], df, dk[d]);
             }
           }
-          if (wk0 + 31 >= klen || qq + 31 >= qlen || (p.causal && dmax > 0)) {
-            // rows that see this lane's key
-            int first = p.causal ? ki - pmin - 4 * hh : -64, last = in ? qlen - qq - 4 * hh : -64;
-            in_branch(first);
-            in_branch(last);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const bool see = acc_row(j, 0) >= first && acc_row(j, 0) < last;
-              pr[j] = see ? pr[j] : 0.f;
-              ds[j] = see ? ds[j] : 0.f;
-            }
-          }
-#pragma unroll
-          for (int tt = 0; tt < 2; ++tt) {
-            frag gc[DB], qc[DB];
-#pragma unroll
-            for (int d = 0; d < DB; ++d) {
-              gc[d] = TL::col(sg, 32 * j2 + 16 * tt, d, lane);
-              qc[d] = TL::col(sq, 32 * j2 + 16 * tt, d, lane);
-            }
-            const frag pf = El<T>::pack(pr + 8 * tt), df = El<T>::pack(ds + 8 * tt);
-#pragma unroll
-            for (int d = 0; d < DB; ++d) {
-              El<T>::mma(gc[d], pf, dv[d]);
-              El<T>::mma(qc[d], df, dk[d]);
-            }
-          }
+        };
+        for (int t = 0; t < ntile; t += 2) {
+          step(t, std::integral_constant<int, 0>());
+          if (t + 1 < ntile) step(t + 1, std::integral_constant<int, 1>());
         }
-      };
-      for (int t = 0; t < ntile; t += 2) {
-        step(t, std::integral_constant<int, 0>());
-        if (t + 1 < ntile) step(t + 1, std::integral_constant<int, 1>());
       }
     }
-  }
-  // rows behind the sequence are zeros whatever the streamed rows hold
-  const int v4 = p.D % 4 == 0;
-  const long half = (long)p.gsplit * p.B * p.Tk * p.Hkv * p.D;
-  auto part = [&](int row) { return p.gpart + ((((long)gpart * p.B + b) * p.Tk + row) * p.Hkv + hk) * p.D; };
-  T* ko = (T*)p.dk + b * p.dks.b + hk * p.dks.h;
-  T* vo = (T*)p.dv + b * p.dvs.b + hk * p.dvs.h;
-  if constexpr (WS == 1) {
-    if (ki >= p.Tk) return;
-    if (p.gsplit > 1) {
-      if (in) {
-        store_rows<float, DP>(part(ki), dk, p.scale, p.D, v4, hh);
-        store_rows<float, DP>(part(ki) + half, dv, 1.f, p.D, v4, hh);
+    // rows behind the sequence are zeros whatever the streamed rows hold
+    const int v4 = D % 4 == 0;
+    const long half = (long)p.gsplit * p.B * p.Tk * p.Hkv * p.D;
+    auto part = [&](int row) { return p.gpart + ((((long)gpart * p.B + b) * p.Tk + row) * p.Hkv + hk) * p.D; };
+    T* ko = (T*)p.dk + b * p.dks.b + hk * p.dks.h;
+    T* vo = (T*)p.dv + b * p.dvs.b + hk * p.dvs.h;
+    if constexpr (WS == 1) {
+      if (ki >= p.Tk) {
+        // no such row
+      } else if (p.gsplit > 1) {
+        if (in) {
+          store_rows<float, DP>(part(ki), dk, p.scale, D, v4, hh);
+          store_rows<float, DP>(part(ki) + half, dv, 1.f, D, v4, hh);
+        } else {
+          zero_rows<float, DP>(part(ki), D, v4, hh);
+          zero_rows<float, DP>(part(ki) + half, D, v4, hh);
+        }
+      } else if (in) {
+        store_rows<T, DP>(ko + (long)ki * p.dks.t, dk, p.scale, D, p.vec, hh);
+        store_rows<T, DP>(vo + (long)ki * p.dvs.t, dv, 1.f, D, p.vec, hh);
       } else {
-        zero_rows<float, DP>(part(ki), p.D, v4, hh);
-        zero_rows<float, DP>(part(ki) + half, p.D, v4, hh);
+        zero_rows<T, DP>(ko + (long)ki * p.dks.t, D, p.vec, hh);
+        zero_rows<T, DP>(vo + (long)ki * p.dvs.t, D, p.vec, hh);
       }
-    } else if (in) {
-      store_rows<T, DP>(ko + (long)ki * p.dks.t, dk, p.scale, p.D, p.vec, hh);
-      store_rows<T, DP>(vo + (long)ki * p.dvs.t, dv, 1.f, p.D, p.vec, hh);
     } else {
-      zero_rows<T, DP>(ko + (long)ki * p.dks.t, p.D, p.vec, hh);
-      zero_rows<T, DP>(vo + (long)ki * p.dvs.t, p.D, p.vec, hh);
+      join<DP, WS>(smem, dk, p.scale, wr, ws, lane, [&](int row, int d, float* x) {
+        if (wk0 + row >= p.Tk) return;
+        if (wk0 + row >= klen) x[0] = x[1] = x[2] = x[3] = 0.f;
+        if (p.gsplit > 1) store4_row(part(wk0 + row), d, x, D, v4);
+        else store4_row(ko + (long)(wk0 + row) * p.dks.t, d, x, D, p.vec);
+      });
+      join<DP, WS>(smem, dv, 1.f, wr, ws, lane, [&](int row, int d, float* x) {
+        if (wk0 + row >= p.Tk) return;
+        if (wk0 + row >= klen) x[0] = x[1] = x[2] = x[3] = 0.f;
+        if (p.gsplit > 1) store4_row(part(wk0 + row) + half, d, x, D, v4);
+        else store4_row(vo + (long)(wk0 + row) * p.dvs.t, d, x, D, p.vec);
+      });
     }
-  } else {
-    join<DP, WS>(smem, dk, p.scale, wr, ws, lane, [&](int row, int d, float* x) {
-      if (wk0 + row >= p.Tk) return;
-      if (wk0 + row >= klen) x[0] = x[1] = x[2] = x[3] = 0.f;
-      if (p.gsplit > 1) store4_row(part(wk0 + row), d, x, p.D, v4);
-      else store4_row(ko + (long)(wk0 + row) * p.dks.t, d, x, p.D, p.vec);
-    });
-    join<DP, WS>(smem, dv, 1.f, wr, ws, lane, [&](int row, int d, float* x) {
-      if (wk0 + row >= p.Tk) return;
-      if (wk0 + row >= klen) x[0] = x[1] = x[2] = x[3] = 0.f;
-      if (p.gsplit > 1) store4_row(part(wk0 + row) + half, d, x, p.D, v4);
-      else store4_row(vo + (long)(wk0 + row) * p.dvs.t, d, x, p.D, p.vec);
-    });
   }
 }
 
-// dk, dv from the head groups' sums, in order
-template <class T> __global__ __launch_bounds__(256) void ba_gsum_kernel(BaParams p) {
-  const long n = (long)p.B * p.Tk * p.Hkv * p.D, i = (long)blockIdx.x * 256 + threadIdx.x;
+// dk, dv from the head groups' sums, in order: four channels a thread, or one where D % 4
+template <class T, int N> __global__ __launch_bounds__(256) void ba_gsum_kernel(BaParams p) {
+  const long n = (long)p.B * p.Tk * p.Hkv * p.D, i = ((long)blockIdx.x * 256 + threadIdx.x) * N;
   if (i >= 2 * n) return;
   const bool second = i >= n;
-  const long e = second ? i - n : i, d = e % p.D, hk = e / p.D % p.Hkv, row = e / p.D / p.Hkv;
+  const long e = second ? i - n : i, row = e / p.D;
   const float* x = p.gpart + (second ? p.gsplit * n : 0) + e;
-  float a = 0.f;
-  for (int g = 0; g < p.gsplit; ++g) a += x[g * n];
+  float a[N];
+#pragma unroll
+  for (int c = 0; c < N; ++c) a[c] = 0.f;
+  for (int g = 0; g < p.gsplit; ++g) {
+    if constexpr (N == 4) {
+      const f32x4 v = *(const f32x4*)(x + g * n);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) a[c] += v[c];
+    } else {
+      a[0] += x[g * n];
+    }
+  }
   const BaStride st = second ? p.dvs : p.dks;
-  ((T*)(second ? p.dv : p.dk))[row / p.Tk * st.b + row % p.Tk * st.t + hk * st.h + d] = (T)a;
+  const long pos = row / p.Hkv;
+  T* out = (T*)(second ? p.dv : p.dk) + pos / p.Tk * st.b + pos % p.Tk * st.t + row % p.Hkv * st.h + e % p.D;
+  if (N == 4 && p.vec) El<T>::store4(out, a);
+  else
+#pragma unroll
+    for (int c = 0; c < N; ++c) out[c] = (T)a[c];
 }
 
 // ---------------------------------------------------------------- launches
-// Rows of a workgroup: 128, or 64 where that leaves fewer than four workgroups a CU, or 32 (spread) where 64 leave every
-// other CU idle (not where the spread form's LDS would not hold the table sums of far borders). dK dV first splits the
+// Rows of a workgroup: 128, or 64 where that leaves fewer than two workgroups' work a CU, or 32 (spread) where 64 leave
+// every other CU idle (not where the spread form's LDS would not hold the table sums of far borders). dK dV first splits the
 // heads of a group.
 constexpr int kSat = 4 * 32 * 4;   // bytes of `sat`, four waves
-struct BwdPlan { int rows_q, rows_k, gsplit, ntq, ntk; };
-int rows_of(long heads, int T) {
-  return heads * ((T + 127) / 128) >= 1024 ? 128 : heads * ((T + 63) / 64) >= 128 ? 64 : 32;
+struct BwdPlan { int rows_q, rows_k, gsplit, ntq, ntk, ranks_k; };
+int rows_of(const BaParams& p, long heads, int T) {
+  const int halves = p.causal ? 2 : 1;   // (a causal workgroup is half as long, or two tiles)
+  return heads * ((T + 127) / 128) >= 512 * halves ? 128 : heads * ((T + 63) / 64) >= 128 * halves ? 64 : 32;
 }
 BwdPlan plan_bwd(const BaParams& p) {
   BwdPlan b;
   const int dp = p.D <= 64 ? 64 : p.D <= 96 ? 96 : 128, spread = 1024 * dp;   // the spread Shape's bytes, any type
-  b.rows_q = rows_of((long)p.B * p.Hq, p.Tq);
+  b.rows_q = rows_of(p, (long)p.B * p.Hq, p.Tq);
   if (b.rows_q == 32 && spread + 5 * host_ext_bytes(p) + kSat > kLds) b.rows_q = 64;
   b.ntq = (p.Tq + b.rows_q - 1) / b.rows_q;
   const long kv = (long)p.B * p.Hkv;
-  b.rows_k = rows_of(kv * p.G, p.Tk);
+  b.rows_k = rows_of(p, kv * p.G, p.Tk);
   b.ntk = (p.Tk + b.rows_k - 1) / b.rows_k;
-  b.gsplit = kv * b.ntk < 512 ? p.G : 1;
+  b.ranks_k = p.causal ? (b.ntk + 1) / 2 : b.ntk;   // paired
+  b.gsplit = 1;
+  while (b.gsplit < p.G && kv * b.ranks_k * b.gsplit < 256)
+    do ++b.gsplit; while (p.G % b.gsplit);
   return b;
 }
 
@@ -507,14 +539,13 @@ template <class T, int DP, int WR> hipError_t bwd_q(BaParams p, const BwdPlan& b
   static_assert(WR > 1 || SH::BYTES == 1024 * DP, "plan_bwd");
   const long grid = (long)p.B * p.Hq * b.ntq;
   p.ntile = b.ntq;
-  p.zigzag = grid <= 512;
   return launch(ba_dq_kernel<T, DP, WR, 4 / WR>, grid, 256, SH::BYTES + 5 * host_ext_bytes(p) + kSat, p, s);
 }
 template <class T, int DP, int WR> hipError_t bwd_k(BaParams p, const BwdPlan& b, hipStream_t s) {
   typedef Shape<T, DP, WR, 4 / WR> SH;
-  const long grid = (long)p.B * p.Hkv * b.gsplit * b.ntk;
+  const long grid = (long)p.B * p.Hkv * b.gsplit * b.ranks_k;
   p.ntile = b.ntk;
-  p.zigzag = grid <= 512;
+  p.pair = p.causal;
   return launch(ba_dkv_kernel<T, DP, WR, 4 / WR>, grid, 256, SH::BYTES + SH::NBUF * 2 * SH::KT * 4 + host_ext_bytes(p), p, s);
 }
 template <class T, int DP> hipError_t bwd(const BaParams& p, const BwdPlan& b, hipStream_t s) {
@@ -523,9 +554,11 @@ template <class T, int DP> hipError_t bwd(const BaParams& p, const BwdPlan& b, h
     e = b.rows_k == 128 ? bwd_k<T, DP, 4>(p, b, s) : b.rows_k == 64 ? bwd_k<T, DP, 2>(p, b, s) : bwd_k<T, DP, 1>(p, b, s);
   if (e != hipSuccess) return e;
   if (p.gsplit > 1) {
-    const long n = 2L * p.B * p.Tk * p.Hkv * p.D, blocks = (n + 255) / 256;
+    const bool four = p.D % 4 == 0;
+    const long n = 2L * p.B * p.Tk * p.Hkv * p.D / (four ? 4 : 1), blocks = (n + 255) / 256;
     if (blocks > 0x7fffffffL) return hipErrorInvalidValue;
-    if (blocks) hipLaunchKernelGGL((ba_gsum_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, p);
+    if (blocks && four) hipLaunchKernelGGL((ba_gsum_kernel<T, 4>), dim3((unsigned)blocks), dim3(256), 0, s, p);
+    else if (blocks) hipLaunchKernelGGL((ba_gsum_kernel<T, 1>), dim3((unsigned)blocks), dim3(256), 0, s, p);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   hipLaunchKernelGGL((ba_dtable_kernel<T>), dim3((unsigned)(p.nb * p.Hq)), dim3(64), 0, s, p.tpart, (long)p.B * b.ntq,

@@ -91,6 +91,9 @@ template <class T> GT_DEV f32x16 mma0(const typename El<T>::frag& a, const typen
 }
 // keeps what follows inside its wave-uniform branch: the compiler would otherwise run such blocks always, with selects
 template <class X> GT_DEV void in_branch(X& x) { asm volatile("" : "+v"(x)); }
+// the value as if computed here: addresses and conditions formed from it are not kept in registers from before a loop
+GT_DEV int anew_v(int x) { asm volatile("" : "+v"(x)); return x; }
+GT_DEV int anew_s(int x) { asm volatile("" : "+s"(x)); return x; }
 GT_DEV void zero16(f32x16& x) {
 #pragma unroll
   for (int j = 0; j < 16; ++j) x[j] = 0.f;
@@ -219,12 +222,9 @@ GT_DEV int start_of(const BaParams& p, int b) {   // far beyond any offset that 
   return s < -(1 << 29) ? -(1 << 29) : s > (1 << 29) ? (1 << 29) : (int)s;
 }
 
-// Work item -> batch, heads and tile. The heads that share a key / value head run next to each other on the same XCD
-// (workgroups go round the 8 XCDs in turn). Tiles: under a causal mask from the longest down; where the whole grid is
-// resident at once, the second half upwards, so that a CU's workgroups add up to about the same work.
-GT_DEV int tile_of(int rank, int ntile, int zigzag) {
-  return zigzag && rank >= (ntile + 1) / 2 ? rank - (ntile + 1) / 2 : ntile - 1 - rank;
-}
+// Work item -> batch, heads and tile: batch entry and key / value head go round first, so that the workgroups that read
+// the same keys run on the same XCD (workgroups go round the 8 XCDs in turn). Under a causal mask a workgroup takes a tile
+// from the end and its mirror image from the start (`pair`): all have the same work, and none runs on alone.
 
 // ---------------------------------------------------------------- streamed rows: global -> LDS
 // Aligned rows go by direct copies to LDS (16 bytes a lane; the lane's slot decides which chunk it fetches, so the image

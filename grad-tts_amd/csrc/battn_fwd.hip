@@ -125,8 +125,6 @@ template <class T> GT_DEV void far_bias(const BaParams& p, int h, Seen& w) {
 }
 
 // ================================================================ shared tiles
-// Under a causal mask a workgroup takes a tile from the end and its mirror image from the start (p.pair): all have the same
-// work, and none runs on alone.
 template <class T, int DP, int WR, int WS>
 __global__ __launch_bounds__(64 * WR * WS, sizeof(T) == 4 ? 1 : 2) void ba_fwd_kernel(BaParams p) {
   typedef Tile<T, DP> TL;
@@ -134,8 +132,7 @@ __global__ __launch_bounds__(64 * WR * WS, sizeof(T) == 4 ? 1 : 2) void ba_fwd_k
   typedef Shape<T, DP, WR, WS> SH;
   constexpr int KT = SH::KT, NB = SH::NB, KS = DP / 16, NT = 64 * WR * WS;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wv % WR, ws = wv / WR;
-  const int r = lane & 31, hh = lane >> 5;
+  const int tid = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wv % WR, ws = wv / WR;
   const int nbk = p.B * p.Hkv, bk = blockIdx.x % (unsigned)nbk, rest = blockIdx.x / (unsigned)nbk, b = bk / p.Hkv, hk = bk % p.Hkv;
   const int h = hk * p.G + rest % p.G, rank = rest / p.G;
   float* ext0 = (float*)(smem + SH::BYTES);
@@ -151,13 +148,13 @@ __global__ __launch_bounds__(64 * WR * WS, sizeof(T) == 4 ? 1 : 2) void ba_fwd_k
     ks.load(tile(t, 0), t * KT);
     vs.load(tile(t, 1), t * KT);
   };
-  if (p.vec && p.D < DP)
-    for (int i = 0; i < 2 * SH::NBUF; ++i) clear_pad<T, DP>(smem + i * SH::TILE, KT, p.D, tid, NT);
   Seen w;
   far_bias<T>(p, h, w);
   w.ext = ext0 + p.dsat + EXT;
   Softmax<T, DP> sm;
+#pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {
+    const int lane = anew_v(tid & 63), r = lane & 31, hh = lane >> 5, D = anew_s(p.D);
     const int tl = pass ? rank : p.ntile - 1 - rank;
     if (pass && (!p.pair || 2 * rank >= p.ntile - 1)) break;
     const int i0 = tl * 32 * WR, wi0 = i0 + 32 * wr, qi = wi0 + r;
@@ -167,8 +164,10 @@ __global__ __launch_bounds__(64 * WR * WS, sizeof(T) == 4 ? 1 : 2) void ba_fwd_k
     if (i0 >= qlen) kend = 0;
     const int ntile = kend > 0 ? (kend + KT - 1) / KT : 0;
     if (pass) __syncthreads();   // the first pass's tiles are done with
+    if (p.vec && D < DP && (WS > 1 || !pass))   // (a join has written over them)
+      for (int i = 0; i < 2 * SH::NBUF; ++i) clear_pad<T, DP>(smem + i * SH::TILE, KT, D, tid, NT);
     frag qf[KS];   // (rows past the last valid one repeat it)
-    if (ntile) load_rows<T, KS>(qf, (const T*)p.q + b * p.qs.b + h * p.qs.h + (long)min(qi, qlen - 1) * p.qs.t, hh, p.D, p.vec);
+    if (ntile) load_rows<T, KS>(qf, (const T*)p.q + b * p.qs.b + h * p.qs.h + (long)min(qi, qlen - 1) * p.qs.t, hh, D, p.vec);
     w.pos = pos0 + qi;
     w.pmin = pos0 + wi0;
     w.pmax = w.pmin + 31;
@@ -214,8 +213,8 @@ __global__ __launch_bounds__(64 * WR * WS, sizeof(T) == 4 ? 1 : 2) void ba_fwd_k
     if constexpr (WS == 1) {
       if (qi >= p.Tq) continue;
       const bool live = in && l != 0.f;
-      if (live) store_rows<T, DP>(ob + (long)qi * p.os.t, sm.o, 1.f / l, p.D, p.vec, hh);
-      else zero_rows<T, DP>(ob + (long)qi * p.os.t, p.D, p.vec, hh);
+      if (live) store_rows<T, DP>(ob + (long)qi * p.os.t, sm.o, 1.f / l, D, p.vec, hh);
+      else zero_rows<T, DP>(ob + (long)qi * p.os.t, D, p.vec, hh);
       if (p.lse && hh == 0) p.lse[stat] = live ? sm.m + __builtin_amdgcn_logf(l) : kInf;
     } else {
       float* sml = ext0 + ext_len(p) + wr * WS * 64;   // [WR][WS][2][32]
@@ -232,7 +231,7 @@ __global__ __launch_bounds__(64 * WR * WS, sizeof(T) == 4 ? 1 : 2) void ba_fwd_k
       join<DP, WS>(smem, sm.o, live ? __builtin_amdgcn_exp2f(sm.m - Mu) / L : 0.f, wr, ws, lane, [&](int row, int d, float* x) {
         if (wi0 + row >= p.Tq) return;
         if (!(wi0 + row < qlen)) x[0] = x[1] = x[2] = x[3] = 0.f;
-        store4_row(ob + (long)(wi0 + row) * p.os.t, d, x, p.D, p.vec);
+        store4_row(ob + (long)(wi0 + row) * p.os.t, d, x, D, p.vec);
       });
     }
   }
@@ -266,7 +265,7 @@ __global__ __launch_bounds__(64 * WSP, sizeof(T) == 2 || DP <= 96 ? 2 : 1) void 
   const unsigned units = (unsigned)nbk * ngb * p.ntile, blk = blockIdx.x % units;   // (the grid is below 2^31)
   const int split = blockIdx.x / units;
   const int bk = blk % (unsigned)nbk, rest = blk / (unsigned)nbk, b = bk / p.Hkv, hk = bk % p.Hkv;
-  const int g0 = rest % ngb * p.gp, i0 = tile_of(rest / ngb, p.ntile, 0) * p.qpb, gp = p.gp;
+  const int g0 = rest % ngb * p.gp, i0 = (p.ntile - 1 - rest / ngb) * p.qpb, gp = p.gp;
   const int qlen = clamp_len(p.qlen, b, p.Tq), klen = clamp_len(p.len, b, p.Tk), pos0 = start_of(p, b);
   float* ext0 = (float*)(smem + SP::BYTES);
   build_ext<T>(p, hk * p.G + g0, gp, hk * p.G + p.G - 1, ext0, tid, NT);
@@ -391,7 +390,7 @@ template <class T> __global__ __launch_bounds__(256) void ba_join_kernel(BaParam
   const int nbk = p.B * p.Hkv, ngb = (p.G + p.gp - 1) / p.gp;
   if (blk >= (long)nbk * ngb * p.ntile) return;
   const int bk = (int)(blk % nbk), rest = (int)(blk / nbk), b = bk / p.Hkv, hk = bk % p.Hkv;
-  const int g = rest % ngb * p.gp + row % p.gp, i = tile_of(rest / ngb, p.ntile, 0) * p.qpb + row / p.gp;
+  const int g = rest % ngb * p.gp + row % p.gp, i = (p.ntile - 1 - rest / ngb) * p.qpb + row / p.gp;
   if (row >= p.gp * p.qpb || g >= p.G || i >= p.Tq) return;
   const float* ml = p.part_ml + blk * p.nsplit * 64 + row;
   float M = -kInf;
@@ -401,14 +400,26 @@ template <class T> __global__ __launch_bounds__(256) void ba_join_kernel(BaParam
   const float Mu = M == -kInf ? 0.f : M;
   float L = 0.f, a0 = 0.f, a1 = 0.f;
   const float* part = p.part + (blk * p.nsplit * 32 + row) * p.D;
-  for (int s = 0; s < p.nsplit; ++s) {
-    const float ls = ml[(long)s * 64 + 32];
-    if (ls == 0.f) continue;   // saw no key (its sums were not written)
-    const float f = __builtin_amdgcn_exp2f(ml[(long)s * 64] - Mu);
-    const float* q = part + (long)s * 32 * p.D;
-    L = __builtin_fmaf(ls, f, L);
-    if (lane < p.D) a0 = __builtin_fmaf(q[lane], f, a0);
-    if (lane + 64 < p.D) a1 = __builtin_fmaf(q[lane + 64], f, a1);
+  const int d0 = min(lane, p.D - 1), d1 = min(lane + 64, p.D - 1);
+  for (int s0 = 0; s0 < p.nsplit; s0 += 8) {   // eight splits' loads together
+    float ms[8], ls[8], x0[8], x1[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const long s = min(s0 + e, p.nsplit - 1);
+      ms[e] = ml[s * 64];
+      ls[e] = ml[s * 64 + 32];
+      x0[e] = part[s * 32 * p.D + d0];
+      x1[e] = part[s * 32 * p.D + d1];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      // a split that saw no key has not written its sums
+      if (s0 + e >= p.nsplit || ls[e] == 0.f) continue;
+      const float f = __builtin_amdgcn_exp2f(ms[e] - Mu);
+      L = __builtin_fmaf(ls[e], f, L);
+      a0 = __builtin_fmaf(x0[e], f, a0);
+      a1 = __builtin_fmaf(x1[e], f, a1);
+    }
   }
   const bool live = i < clamp_len(p.qlen, b, p.Tq) && L != 0.f;
   const int h = hk * p.G + g;
