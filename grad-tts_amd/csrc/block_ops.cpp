@@ -101,7 +101,7 @@ const char* plan_attention(const gt_bucket_attention* a, BaParams& p) {
 
 const char* plan_norm(const gt_residual_norm* a, RnParams& p) {
   if (a->dtype < GT_ELEM_F32 || a->dtype > GT_ELEM_F16) return "dtype must be GT_ELEM_F32, GT_ELEM_BF16 or GT_ELEM_F16";
-  if (a->B < 0 || a->T < 0 || a->B > kMaxT || a->T > kMaxT) return "B and T must lie in [0, 2^28]";
+  if (a->B < 0 || a->T < 0 || a->B > 65535 || a->T > kMaxT) return "B must lie in [0, 65535], T in [0, 2^28]";
   if (a->C < 1 || a->C > RN_MAX_C) return "C must lie in [1, 8192]";
   if (!(a->eps >= 0.f) || !std::isfinite(a->eps) || !std::isfinite(a->scale)) return "eps must be >= 0, eps and scale finite";
   if (!a->post_weight || !a->pre_weight || (a->B * a->T && (!a->x || !a->y))) return "null tensor";

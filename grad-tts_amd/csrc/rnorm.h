@@ -21,8 +21,8 @@ struct RnParams {
   const void *dout, *dh;
   void *dx, *dy;
   float *dgate, *dw1, *db1, *dw2, *db2;   // dgate [C] or [B][C]; dgate, db1, db2 may be null
-  float* part;                       // [B][chunks][4][C]
-  int rows_per_chunk, chunks;        // of one batch entry
+  float *part, *part2;               // [B][chunks][4][C]; [B][ranges][4][C]
+  int rows_per_chunk, chunks, ranges;   // of one batch entry; ranges of its chunks
 };
 
 size_t rn_backward_ws(const RnParams& p);

@@ -70,15 +70,21 @@ template <class T, int TPR, int NC, bool VEC> GT_DEV void row_store(T* p, const 
   }
 }
 
+// sum over the wave in registers (row rotations, then swaps of 16- and 32-lane rows): no LDS round trip a step
+GT_DEV float wave_total(float x) {
+  x = row_sum16(x);
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
 // sums over the TPR threads of a row group; every thread gets them, in one order
 template <int TPR, int N> struct RowSum {
   float* s;   // [2][TPR / 64][N] for this group
   int flip;
   GT_DEV void operator()(float (&v)[N], int t) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) v[i] += __shfl_xor(v[i], o);
+    for (int i = 0; i < N; ++i) v[i] = wave_total(v[i]);
     if constexpr (TPR > 64) {
       constexpr int NW = TPR / 64;
       float* b = s + flip * NW * N;
@@ -294,65 +300,79 @@ __global__ __launch_bounds__(kThreads<TPR>) void rn_bwd_kernel(RnParams p) {
   }
 }
 
-// Column sums of the chunks: 64 channels a workgroup, 16 waves over the chunks of a batch entry, then across the waves
-// and the entries in a fixed order. blockIdx.y 0: d u1, d -> dgate, dw1, db1; 1: dh u2, dh -> dw2, db2.
-__global__ __launch_bounds__(1024) void rn_cols_kernel(RnParams p) {
-  __shared__ float s[2][16][64];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, c = blockIdx.x * 64 + lane, pair = blockIdx.y * 2;
-  float tot0 = 0.f, tot1 = 0.f, dg = 0.f;
+// Column sums of the chunks in two steps, in a fixed order: 64 channels and a range of one batch entry's chunks a workgroup
+// (blockIdx.y: range, blockIdx.z: entry), then all ranges and entries.
+__global__ __launch_bounds__(256) void rn_cols_kernel(RnParams p) {
+  __shared__ float s[4][4][64];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+  const int per = (p.chunks + p.ranges - 1) / p.ranges, k0 = blockIdx.y * per, k1 = min(p.chunks, k0 + per);
+  float a[4] = {0.f, 0.f, 0.f, 0.f};
+  if (c < p.C)
+    for (int k = k0 + wv; k < k1; k += 4) {
+      const float* q = p.part + ((long)blockIdx.z * p.chunks + k) * 4 * p.C + c;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] += q[(long)i * p.C];
+    }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s[wv][i][lane] = a[i];
+  __syncthreads();
+  // wave i adds up column sum i
+  if (c < p.C)
+    p.part2[(((long)blockIdx.z * p.ranges + blockIdx.y) * 4 + wv) * p.C + c] = s[0][wv][lane] + s[1][wv][lane] + s[2][wv][lane] + s[3][wv][lane];
+}
+// sums of d u1, d -> dgate, dw1, db1; of dh u2, dh -> dw2, db2
+__global__ __launch_bounds__(1024) void rn_params_kernel(RnParams p) {
+  __shared__ float s[5][16][64];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
   const bool in = c < p.C;
   const float w1 = in ? p.w1[c] : 0.f, b1 = in && p.b1 ? p.b1[c] : 0.f;
-  for (int b = 0; b < p.B; ++b) {
-    float a0 = 0.f, a1 = 0.f;
-    if (in)
-      for (int k = wv; k < p.chunks; k += 16) {
-        const float* q = p.part + (((long)b * p.chunks + k) * 4 + pair) * p.C + c;
-        a0 += q[0];
-        a1 += q[p.C];
-      }
-    __syncthreads();
-    s[0][wv][lane] = a0;
-    s[1][wv][lane] = a1;
-    __syncthreads();
-    if (wv == 0 && in) {
-      a0 = a1 = 0.f;
-      for (int w = 0; w < 16; ++w) { a0 += s[0][w][lane]; a1 += s[1][w][lane]; }
-      if (pair) { tot0 += a0; tot1 += a1; }
-      else {
-        const float g = p.scale * (p.gate ? p.gate[(p.gate_batch ? (long)b * p.C : 0) + c] : 1.f);
-        tot0 = __builtin_fmaf(g, a0, tot0);
-        tot1 = __builtin_fmaf(g, a1, tot1);
-        const float x = p.scale * (w1 * a0 + b1 * a1);
-        if (p.dgate && p.gate_batch) p.dgate[(long)b * p.C + c] = x;
-        dg += x;
-      }
+  float t[5] = {0.f, 0.f, 0.f, 0.f, 0.f};   // dw1, db1, dw2, db2, dgate
+  if (in)
+    for (int b = wv; b < p.B; b += 16) {   // a wave every sixteenth entry
+      float a[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int r = 0; r < p.ranges; ++r)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] += p.part2[(((long)b * p.ranges + r) * 4 + i) * p.C + c];
+      const float g = p.scale * (p.gate ? p.gate[(p.gate_batch ? (long)b * p.C : 0) + c] : 1.f);
+      t[0] = __builtin_fmaf(g, a[0], t[0]);
+      t[1] = __builtin_fmaf(g, a[1], t[1]);
+      t[2] += a[2];
+      t[3] += a[3];
+      const float x = p.scale * (w1 * a[0] + b1 * a[1]);
+      if (p.dgate && p.gate_batch) p.dgate[(long)b * p.C + c] = x;
+      t[4] += x;
     }
-  }
-  if (wv != 0 || !in) return;
-  if (pair) {
-    p.dw2[c] = tot0;
-    if (p.db2) p.db2[c] = tot1;
-  } else {
-    p.dw1[c] = tot0;
-    if (p.db1) p.db1[c] = tot1;
-    if (p.dgate && !p.gate_batch) p.dgate[c] = dg;
-  }
+#pragma unroll
+  for (int i = 0; i < 5; ++i) s[i][wv][lane] = t[i];
+  __syncthreads();
+  float* out[5] = {p.dw1, p.db1, p.dw2, p.db2, p.gate_batch ? nullptr : p.dgate};
+#pragma unroll
+  for (int i = 0; i < 5; ++i)
+    if (wv == i && in && out[i]) {
+      float a = 0.f;
+      for (int w = 0; w < 16; ++w) a += s[i][w][lane];
+      out[i][c] = a;
+    }
 }
 
 // ---------------------------------------------------------------- launches
 // threads of a row, 8 channels each
 int tpr_of(int C) { return C <= 512 ? 64 : C <= 1024 ? 128 : C <= 2048 ? 256 : C <= 4096 ? 512 : 1024; }
 
-// chunks of a batch entry: about 256 CUs x 1024 threads in all, at least 4 rows each
-void set_chunks(RnParams& p) {
-  const long groups = 262144 / tpr_of(p.C), rows = (long)p.B * p.T;
-  p.rows_per_chunk = p.chunks = 0;
+// chunks of a batch entry: about 256 CUs x 1024 threads in all, the rows of the backward's column sums too (its 156
+// registers leave room for 768), at least 4 rows each
+void set_chunks(RnParams& p, bool bwd) {
+  const long groups = (bwd ? 196608 : 262144) / tpr_of(p.C), rows = (long)p.B * p.T;
+  p.rows_per_chunk = p.chunks = p.ranges = 0;
   if (rows == 0) return;
   long rpc = (rows + groups - 1) / groups;
   if (rpc < 4) rpc = 4;
   if (rpc > p.T) rpc = p.T;
   p.rows_per_chunk = (int)rpc;
   p.chunks = (int)((p.T + rpc - 1) / rpc);
+  // ranges: about 512 workgroups of column sums, 8 chunks each at least
+  const long blocks = (long)((p.C + 63) / 64) * p.B, want = (512 + blocks - 1) / blocks, most = (p.chunks + 7) / 8;
+  p.ranges = (int)(want < most ? want : most);
 }
 
 template <class T, int TPR, int NC, bool VEC> hipError_t go(const RnParams& p, bool bwd, hipStream_t s) {
@@ -382,19 +402,25 @@ hipError_t go_t(const RnParams& p, int dtype, bool bwd, hipStream_t s) {
 
 size_t rn_backward_ws(const RnParams& p0) {
   RnParams p = p0;
-  set_chunks(p);
-  return (size_t)p.B * p.chunks * 4 * p.C * 4 + 256;
+  set_chunks(p, true);
+  return (size_t)p.B * (p.chunks + p.ranges) * 4 * p.C * 4 + 256;
 }
 hipError_t launch_rn_forward(RnParams p, int dtype, hipStream_t s) {
-  set_chunks(p);
+  set_chunks(p, false);
   return p.chunks ? go_t(p, dtype, false, s) : hipSuccess;
 }
 hipError_t launch_rn_backward(RnParams p, int dtype, void* ws, hipStream_t s) {
-  set_chunks(p);
+  set_chunks(p, true);
   p.part = (float*)(((uintptr_t)ws + 255) & ~(uintptr_t)255);
-  if (p.chunks)
+  p.part2 = p.part + (size_t)p.B * p.chunks * 4 * p.C;
+  const unsigned cols = (unsigned)((p.C + 63) / 64);
+  if (p.chunks) {
+    if (p.B > 65535) return hipErrorInvalidValue;   // (block_ops.cpp refuses it)
     if (hipError_t e = go_t(p, dtype, true, s)) return e;
-  rn_cols_kernel<<<dim3((unsigned)((p.C + 63) / 64), 2), dim3(1024), 0, s>>>(p);
+    rn_cols_kernel<<<dim3(cols, (unsigned)p.ranges, (unsigned)p.B), dim3(256), 0, s>>>(p);
+    if (hipError_t e = hipGetLastError()) return e;
+  }
+  rn_params_kernel<<<dim3(cols), dim3(1024), 0, s>>>(p);
   return hipGetLastError();
 }
 
