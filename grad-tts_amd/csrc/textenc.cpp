@@ -3,6 +3,7 @@
 // and the launch sequence of textenc.hip in the reference's order of operations.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <map>
@@ -19,6 +20,7 @@ using namespace gt;
 
 struct gt_text_encoder {
   int n_vocab, n_feats, C, Fc, Fdp, H, L, K, W;
+  int buckets = 0, max_distance = 0;   // bucket form: layers of bucket attention and residual steps; 0: window form
   std::vector<std::pair<std::string, std::vector<int64_t>>> inv;
   std::map<std::string, int> index;
   std::vector<std::vector<float>> host;
@@ -63,18 +65,23 @@ void build_inventory(gt_text_encoder* e) {
   add("prenet.proj.weight", {C, C, 1}); add("prenet.proj.bias", {C});
   for (int l = 0; l < e->L; ++l) {
     const std::string p = "encoder.attn_layers." + std::to_string(l) + ".";
-    add(p + "emb_rel_k", {1, nw, kc}); add(p + "emb_rel_v", {1, nw, kc});
+    if (e->buckets) add(p + "table", {e->buckets, e->H});
+    else { add(p + "emb_rel_k", {1, nw, kc}); add(p + "emb_rel_v", {1, nw, kc}); }
     for (const char* n : {"conv_q", "conv_k", "conv_v", "conv_o"}) { add(p + n + ".weight", {C, C, 1}); add(p + n + ".bias", {C}); }
   }
-  for (int l = 0; l < e->L; ++l) { add("encoder.norm_layers_1." + std::to_string(l) + ".gamma", {C});
-                                    add("encoder.norm_layers_1." + std::to_string(l) + ".beta", {C}); }
+  auto norms = [&](const std::string& k) {
+    for (int l = 0; l < e->L; ++l) { add(k + std::to_string(l) + ".gamma", {C}); add(k + std::to_string(l) + ".beta", {C}); }
+  };
+  if (e->buckets) { add("encoder.norm_in.gamma", {C}); add("encoder.norm_in.beta", {C});
+                    norms("encoder.norm_post_1."); norms("encoder.norm_pre_1."); }
+  else norms("encoder.norm_layers_1.");
   for (int l = 0; l < e->L; ++l) {
     const std::string p = "encoder.ffn_layers." + std::to_string(l) + ".";
     add(p + "conv_1.weight", {e->Fc, C, e->K}); add(p + "conv_1.bias", {e->Fc});
     add(p + "conv_2.weight", {C, e->Fc, e->K}); add(p + "conv_2.bias", {C});
   }
-  for (int l = 0; l < e->L; ++l) { add("encoder.norm_layers_2." + std::to_string(l) + ".gamma", {C});
-                                    add("encoder.norm_layers_2." + std::to_string(l) + ".beta", {C}); }
+  if (e->buckets) { norms("encoder.norm_post_2."); norms("encoder.norm_pre_2."); }
+  else norms("encoder.norm_layers_2.");
   add("proj_m.weight", {e->n_feats, C, 1}); add("proj_m.bias", {e->n_feats});
   add("proj_w.conv_1.weight", {e->Fdp, C, e->K}); add("proj_w.conv_1.bias", {e->Fdp});
   add("proj_w.norm_1.gamma", {e->Fdp}); add("proj_w.norm_1.beta", {e->Fdp});
@@ -141,8 +148,45 @@ int upload(gt_text_encoder* e) {
   return GT_OK;
 }
 
+// ---- bucket form: the blocks' operators on the encoder's tensors
+// attention of all heads on qkv [B][T][3C] (q | k | v), bidirectional, keys and queries of the lengths only
+gt_bucket_attention attn_args(const gt_text_encoder* e, int64_t B, int64_t T, const float* qkv, const float* table,
+                              const int64_t* lengths) {
+  const int64_t C = e->C, D = e->C / e->H;
+  gt_bucket_attention a{};
+  a.dtype = GT_ELEM_F32; a.n_buckets = e->buckets; a.max_distance = e->max_distance;
+  a.scale = 1.f / std::sqrt((float)D);
+  a.B = B; a.Tq = a.Tk = T; a.Hq = a.Hkv = e->H; a.D = D;
+  a.q = qkv; a.k = qkv + C; a.v = qkv + 2 * C; a.table = table;
+  a.q_stride = a.k_stride = a.v_stride = {3 * C * T, 3 * C, D};
+  a.out_stride = {C * T, C, D};
+  a.lengths = a.q_lengths = lengths;
+  return a;
+}
+// out = x + N_post(y), h = N_pre(out); the parameters are gamma | beta in `post` and `pre`
+gt_residual_norm step_args(const gt_text_encoder* e, int64_t B, int64_t T, const float* x, const float* y,
+                           const float* post, const float* pre, const int64_t* lengths) {
+  gt_residual_norm a{};
+  a.dtype = GT_ELEM_F32; a.scale = 1.f; a.eps = 1e-4f;
+  a.B = B; a.T = T; a.C = e->C; a.x = x; a.y = y;
+  a.post_weight = post; a.post_bias = post + e->C; a.pre_weight = pre; a.pre_bias = pre + e->C;
+  a.lengths = lengths;
+  return a;
+}
+// their workspaces (sizes depend on shapes alone; the addresses stand for aligned buffers)
+size_t attn_ws_bytes(const gt_text_encoder* e, int64_t B, int64_t T, bool backward) {
+  const float* some = (const float*)(uintptr_t)4096;
+  const gt_bucket_attention a = attn_args(e, B, T, some, some, nullptr);
+  return backward ? gt_bucket_attention_backward_workspace_bytes(&a) : gt_bucket_attention_workspace_bytes(&a);
+}
+size_t step_ws_bytes(const gt_text_encoder* e, int64_t B, int64_t T) {
+  const float* some = (const float*)(uintptr_t)4096;
+  const gt_residual_norm a = step_args(e, B, T, some, some, some, some, nullptr);
+  return gt_residual_norm_backward_workspace_bytes(&a);
+}
+
 struct Ws {   // workspace layout (floats), 256-byte aligned pieces
-  size_t x0, xa, xb, x1, hid, qkv, att, d1, d2, total;
+  size_t x0, xa, xb, x1, hid, qkv, att, d1, d2, blk, blk_bytes, total;
 };
 Ws ws_layout(const gt_text_encoder* e, int64_t B, int64_t T) {
   Ws w{};
@@ -152,6 +196,10 @@ Ws ws_layout(const gt_text_encoder* e, int64_t B, int64_t T) {
   w.x0 = put(n * e->C); w.xa = put(n * e->C); w.xb = put(n * e->C); w.x1 = put(n * e->C);
   w.hid = put(n * e->Fc); w.qkv = put(n * 3 * e->C); w.att = put(n * e->C);
   w.d1 = put(n * e->Fdp); w.d2 = put(n * e->Fdp);
+  if (e->buckets) {
+    w.blk_bytes = attn_ws_bytes(e, B, T, false);
+    w.blk = put((w.blk_bytes + 3) / 4);
+  }
   w.total = off + 256;
   return w;
 }
@@ -175,6 +223,26 @@ int gt_text_encoder_create(int n_vocab, int n_feats, int n_channels, int filter_
   *out = e;
   return GT_OK;
 }
+
+int gt_text_encoder_create_buckets(int n_vocab, int n_feats, int n_channels, int filter_channels,
+                                   int filter_channels_dp, int n_heads, int n_layers, int kernel_size, int n_buckets,
+                                   int max_distance, gt_text_encoder** out) try {
+  if (!out) return gt_internal_fail(GT_ERR_ARG, "null out");
+  *out = nullptr;
+  if (n_vocab <= 0 || n_feats <= 0 || n_feats > 128 || n_layers <= 0 || filter_channels <= 0 || filter_channels_dp <= 0 ||
+      filter_channels_dp > 256 || kernel_size < 1 || kernel_size > 5 || kernel_size % 2 == 0 || n_heads <= 0 ||
+      n_channels <= 0 || n_channels > 256 || n_channels % n_heads || n_channels / n_heads > 128)
+    return gt_internal_fail(GT_ERR_UNSUPPORTED, "text encoder kernels implement heads of <= 128 channels, <= 256 channels "
+                                                "in LayerNorms, odd kernels <= 5, <= 128 features");
+  if (gt_relative_bucket(0, n_buckets, max_distance, 0) < 0)
+    return gt_internal_fail(GT_ERR_ARG, "n_buckets must be even in [4, 128], max_distance in (n_buckets / 4, 1024]");
+  gt_text_encoder* e = new gt_text_encoder();
+  e->n_vocab = n_vocab; e->n_feats = n_feats; e->C = n_channels; e->Fc = filter_channels; e->Fdp = filter_channels_dp;
+  e->H = n_heads; e->L = n_layers; e->K = kernel_size; e->W = 0; e->buckets = n_buckets; e->max_distance = max_distance;
+  build_inventory(e);
+  *out = e;
+  return GT_OK;
+} catch (...) { return gt_internal_fail(GT_ERR_ARG, "gt_text_encoder_create_buckets: out of memory"); }
 
 void gt_text_encoder_destroy(gt_text_encoder* e) {
   if (!e) return;
@@ -290,8 +358,38 @@ int gt_text_encoder_forward(gt_text_encoder* e, const int64_t* tokens, const int
   }
   float* x = x1;
   conv(h, C, C, nullptr, "prenet.proj", C, 1, x, C, 0, 0, x0, x_mask, 0);   // (x_org + proj(x)) * x_mask
+  // bucket form: h = N(x) into the first layer; per layer x += N_post(block(h)), h = N_pre(x) for the attention and
+  // the FFN; the encoder's output is the last h. x, h are zero behind the lengths.
+  int rc_blk = GT_OK;
+  if (e->buckets) {
+    float *xs = x1, *xo = x0, *hb = xb;
+    ln(xs, nullptr, "encoder.norm_in", C, 0, x_mask, hb);
+    auto step = [&](const std::string& i, int l) {
+      const std::string t = std::to_string(l) + ".gamma";
+      const gt_residual_norm a = step_args(e, B, T, xs, xa, P("encoder.norm_post_" + i + "." + t),
+                                           P("encoder.norm_pre_" + i + "." + t), x_lengths);
+      if (!rc_blk) rc_blk = gt_residual_norm_forward(&a, xo, hb, nullptr, stream);
+      std::swap(xs, xo);
+    };
+    for (int l = 0; l < e->L; ++l) {
+      const std::string a = "encoder.attn_layers." + std::to_string(l) + ".";
+      conv(hb, C, C, nullptr, a + "conv_q", C, 1, qkv, 3 * C, 0, 0, nullptr, nullptr, 0);
+      conv(hb, C, C, nullptr, a + "conv_k", C, 1, qkv, 3 * C, C, 0, nullptr, nullptr, 0);
+      conv(hb, C, C, nullptr, a + "conv_v", C, 1, qkv, 3 * C, 2 * C, 0, nullptr, nullptr, 0);
+      const gt_bucket_attention b = attn_args(e, B, T, qkv, P(a + "table"), x_lengths);
+      if (!rc_blk) rc_blk = gt_bucket_attention_forward(&b, att, nullptr, buf(w.blk), w.blk_bytes, stream);
+      conv(att, C, C, nullptr, a + "conv_o", C, 1, xa, C, 0, 0, nullptr, nullptr, 0);
+      step("1", l);
+      const std::string f = "encoder.ffn_layers." + std::to_string(l) + ".";
+      conv(hb, C, C, x_mask, f + "conv_1", e->Fc, e->K, hid, e->Fc, 0, 1, nullptr, nullptr, 0);
+      conv(hid, e->Fc, e->Fc, x_mask, f + "conv_2", C, e->K, xa, C, 0, 0, nullptr, x_mask, 0);
+      step("2", l);
+    }
+    x = hb;
+    if (rc_blk) return rc_blk;
+  }
   // encoder layers (:271-282); x is masked on entry to every layer
-  for (int l = 0; l < e->L; ++l) {
+  for (int l = 0; l < e->L && !e->buckets; ++l) {
     const std::string a = "encoder.attn_layers." + std::to_string(l) + ".";
     conv(x, C, C, nullptr, a + "conv_q", C, 1, qkv, 3 * C, 0, 0, nullptr, nullptr, 0);
     conv(x, C, C, nullptr, a + "conv_k", C, 1, qkv, 3 * C, C, 0, nullptr, nullptr, 0);
@@ -371,6 +469,9 @@ namespace {
 struct TrWs {
   size_t tokens, mask, x0, pre_c[3], pre_h[3], x1, d1c, d1d, d2c, d2d;
   std::vector<size_t> qkv, P, Pd, PdT, att, y1, xmid, hd, y2, xout;
+  // bucket form: h into the first layer, the layers' streams and statistics, the stream's gradient, lengths
+  std::vector<size_t> lse, o1, o2, st1, st2;
+  size_t h0, sa, sb, lengths, blk, blk_bytes;
   size_t g1, g2, datt, dy, dh, dqkv, ds, dsT, drel, wpart, cpart, lpart, dmu;
   long wpart_floats, cpart_floats;
   size_t total;
@@ -393,15 +494,26 @@ TrWs tr_layout(const gt_text_encoder* e, int64_t B, int64_t T) {
   for (int i = 0; i < 3; ++i) { w.pre_c[i] = put(n * C); w.pre_h[i] = put(n * C); }
   w.x1 = put(n * C);
   for (int l = 0; l < e->L; ++l) {
-    w.qkv.push_back(put(n * 3 * C)); w.P.push_back(put(att)); w.Pd.push_back(put(att)); w.PdT.push_back(put(att));
+    w.qkv.push_back(put(n * 3 * C));
+    if (e->buckets) {
+      w.lse.push_back(put(n * e->H)); w.o1.push_back(put(n * C)); w.o2.push_back(put(n * C));
+      w.st1.push_back(put(n * 4)); w.st2.push_back(put(n * 4));
+    } else { w.P.push_back(put(att)); w.Pd.push_back(put(att)); w.PdT.push_back(put(att)); }
     w.att.push_back(put(n * C)); w.y1.push_back(put(n * C)); w.xmid.push_back(put(n * C));
     w.hd.push_back(put(n * Fc)); w.y2.push_back(put(n * C)); w.xout.push_back(put(n * C));
   }
   w.d1c = put(n * Fd); w.d1d = put(n * Fd); w.d2c = put(n * Fd); w.d2d = put(n * Fd);
   const size_t wide = std::max({C, Fc, Fd, (size_t)e->n_feats});
   w.g1 = put(n * C); w.g2 = put(n * C); w.datt = put(n * C);
-  w.dy = put(n * wide); w.dh = put(n * wide); w.dqkv = put(n * 3 * C); w.ds = put(att); w.dsT = put(att);
-  w.drel = put((size_t)B * 2 * (2 * e->W + 1) * 96);
+  w.dy = put(n * wide); w.dh = put(n * wide); w.dqkv = put(n * 3 * C);
+  if (e->buckets) {
+    w.h0 = put(n * C); w.sa = put(n * C); w.sb = put(n * C); w.lengths = put(2 * (size_t)B);
+    w.blk_bytes = std::max({attn_ws_bytes(e, B, T, false), attn_ws_bytes(e, B, T, true), step_ws_bytes(e, B, T)});
+    w.blk = put((w.blk_bytes + 3) / 4);
+  } else {
+    w.ds = put(att); w.dsT = put(att);
+    w.drel = put((size_t)B * 2 * (2 * e->W + 1) * 96);
+  }
   w.wpart_floats = 8L << 20;
   w.wpart = put((size_t)w.wpart_floats);
   w.cpart_floats = 64L * (long)wide;
@@ -490,7 +602,43 @@ int gt_text_encoder_forward_train(gt_text_encoder* e, const int64_t* tokens, con
   }
   conv(h, C, nullptr, "prenet.proj", C, 1, F(w.x1), C, 0, 0, F(w.x0), mask, 0, none);
   const float* x = F(w.x1);
-  for (int l = 0; l < e->L; ++l) {
+  if (e->buckets) {   // as in the inference pass; the attention's probabilities are never stored and take no dropout
+    const int64_t* lens = (const int64_t*)F(w.lengths);
+    chk(launch_tt_copy_words((uint32_t*)F(w.lengths), (const uint32_t*)x_lengths, 2 * (long)B, s));
+    ln(x, nullptr, "encoder.norm_in", C, 0, mask, F(w.h0), none);
+    const float* h = F(w.h0);
+    int rc_blk = GT_OK;
+    auto step = [&](const std::string& i, int l, size_t y, size_t out, size_t hn, size_t st) {
+      const std::string t = std::to_string(l) + ".gamma";
+      const gt_residual_norm a = step_args(e, B, T, x, F(y), P("encoder.norm_post_" + i + "." + t),
+                                           P("encoder.norm_pre_" + i + "." + t), lens);
+      if (!rc_blk) rc_blk = gt_residual_norm_forward(&a, F(out), F(hn), F(st), stream);
+      x = F(out);
+      h = F(hn);
+    };
+    for (int l = 0; l < e->L; ++l) {
+      const std::string a = "encoder.attn_layers." + std::to_string(l) + ".";
+      const std::string f = "encoder.ffn_layers." + std::to_string(l) + ".";
+      const uint32_t site = 16 + 8 * l;
+      float* qkv = F(w.qkv[l]);
+      conv(h, C, nullptr, a + "conv_q", C, 1, qkv, 3 * C, 0, 0, nullptr, nullptr, 0, none);
+      conv(h, C, nullptr, a + "conv_k", C, 1, qkv, 3 * C, C, 0, nullptr, nullptr, 0, none);
+      conv(h, C, nullptr, a + "conv_v", C, 1, qkv, 3 * C, 2 * C, 0, nullptr, nullptr, 0, none);
+      const gt_bucket_attention b = attn_args(e, B, T, qkv, P(a + "table"), lens);
+      if (!rc_blk) rc_blk = gt_bucket_attention_forward(&b, F(w.att[l]), F(w.lse[l]), F(w.blk), w.blk_bytes, stream);
+      conv(F(w.att[l]), C, nullptr, a + "conv_o", C, 1, F(w.y1[l]), C, 0, 0, nullptr, nullptr, 0,
+           make_drop(seed, site + 1, p_dropout));
+      step("1", l, w.y1[l], w.o1[l], w.xmid[l], w.st1[l]);
+      conv(h, C, mask, f + "conv_1", e->Fc, e->K, F(w.hd[l]), e->Fc, 0, 1, nullptr, nullptr, 0,
+           make_drop(seed, site + 2, p_dropout));
+      conv(F(w.hd[l]), e->Fc, mask, f + "conv_2", C, e->K, F(w.y2[l]), C, 0, 0, nullptr, mask, 0,
+           make_drop(seed, site + 3, p_dropout));
+      step("2", l, w.y2[l], w.o2[l], w.xout[l], w.st2[l]);
+    }
+    x = h;
+    if (rc_blk) return rc_blk;
+  }
+  for (int l = 0; l < e->L && !e->buckets; ++l) {
     const std::string a = "encoder.attn_layers." + std::to_string(l) + ".";
     const std::string f = "encoder.ffn_layers." + std::to_string(l) + ".";
     const uint32_t site = 16 + 8 * l;
@@ -622,8 +770,57 @@ int gt_text_encoder_backward(gt_text_encoder* e, const float* dmu_x, const float
   ew(DMU, NF, dmu_x, NF, 1, NF, mask, none, nullptr, 0);
   wgrad(DMU, NF, xf, C, nullptr, "proj_m", NF, C, 1);
   dgrad(DMU, NF, "proj_m", NF, C, 1, G1, C, 0, mask);
+  // ---- bucket form: G1 = dL/dh, SA = dL/dx of the stream, both zero behind the lengths
+  if (e->buckets) {
+    const int64_t* lens = (const int64_t*)F(w.lengths);
+    float *SA = F(w.sa), *SB = F(w.sb);
+    int rc_blk = GT_OK;
+    ew(SA, C, nullptr, C, 0, C, mask, none, nullptr, 0);   // the last x is read by its norm alone: zeros
+    auto step = [&](const std::string& i, int l, const float* x, size_t y, size_t st, const float* dout, const float* dh,
+                    float* dx, float* dyo) {
+      const std::string post = "encoder.norm_post_" + i + "." + std::to_string(l);
+      const std::string pre = "encoder.norm_pre_" + i + "." + std::to_string(l);
+      const gt_residual_norm a = step_args(e, B, T, x, F(y), P(post + ".gamma"), P(pre + ".gamma"), lens);
+      gt_residual_norm_grads g{};
+      g.dout = dout; g.dh = dh; g.dx = dx; g.dy = dyo;
+      g.dpost_weight = G(post + ".gamma"); g.dpost_bias = G(post + ".beta");
+      g.dpre_weight = G(pre + ".gamma"); g.dpre_bias = G(pre + ".beta");
+      if (!rc_blk) rc_blk = gt_residual_norm_backward(&a, F(st), &g, F(w.blk), w.blk_bytes, stream);
+    };
+    for (int l = e->L - 1; l >= 0; --l) {
+      const std::string a = "encoder.attn_layers." + std::to_string(l) + ".";
+      const std::string f = "encoder.ffn_layers." + std::to_string(l) + ".";
+      const uint32_t site = 16 + 8 * l;
+      const float* hin = l ? F(w.xout[l - 1]) : F(w.h0);
+      step("2", l, F(w.o1[l]), w.y2[l], w.st2[l], SA, G1, SB, G2);
+      ew(DY, C, G2, C, 0, C, mask, make_drop(seed, site + 3, pd), nullptr, 0);
+      wgrad(DY, C, F(w.hd[l]), Fc, mask, f + "conv_2", C, Fc, K);
+      dgrad(DY, C, f + "conv_2", C, Fc, K, DH, Fc, 0, nullptr);
+      ew(DH, Fc, DH, Fc, 0, Fc, mask, make_drop(seed, site + 2, pd), F(w.hd[l]), Fc);
+      wgrad(DH, Fc, F(w.xmid[l]), C, mask, f + "conv_1", Fc, C, K);
+      dgrad(DH, Fc, f + "conv_1", Fc, C, K, G2, C, 0, mask);
+      step("1", l, l ? F(w.o2[l - 1]) : F(w.x1), w.y1[l], w.st1[l], SB, G2, SA, G1);
+      ew(DY, C, G1, C, 0, C, mask, make_drop(seed, site + 1, pd), nullptr, 0);
+      wgrad(DY, C, F(w.att[l]), C, nullptr, a + "conv_o", C, C, 1);
+      dgrad(DY, C, a + "conv_o", C, C, 1, DATT, C, 0, nullptr);
+      const gt_bucket_attention b = attn_args(e, B, T, F(w.qkv[l]), P(a + "table"), lens);
+      gt_bucket_attention_grads g{};
+      g.dout = DATT; g.dq = DQKV; g.dk = DQKV + C; g.dv = DQKV + 2 * C; g.dtable = G(a + "table");
+      g.dout_stride = b.out_stride;
+      g.dq_stride = g.dk_stride = g.dv_stride = b.q_stride;
+      if (!rc_blk) rc_blk = gt_bucket_attention_backward(&b, F(w.att[l]), F(w.lse[l]), &g, F(w.blk), w.blk_bytes, stream);
+      const char* qkvn[3] = {"conv_q", "conv_k", "conv_v"};
+      for (int j = 0; j < 3; ++j) {
+        wgrad(DQKV + j * C, 3 * C, hin, C, nullptr, a + qkvn[j], C, C, 1);
+        dgrad(DQKV + j * C, 3 * C, a + qkvn[j], C, C, 1, G1, C, j > 0, mask);
+      }
+    }
+    lnb(F(w.x1), nullptr, "encoder.norm_in", C, G1, none, nullptr, 0, SA, 1, mask);
+    ew(G1, C, SA, C, 0, C, mask, none, nullptr, 0);
+    if (rc_blk) return rc_blk;
+  }
   // ---- encoder layers, last to first; G1 = dL/d(layer output), masked
-  for (int l = e->L - 1; l >= 0; --l) {
+  for (int l = e->L - 1; l >= 0 && !e->buckets; --l) {
     const std::string a = "encoder.attn_layers." + std::to_string(l) + ".";
     const std::string f = "encoder.ffn_layers." + std::to_string(l) + ".";
     const uint32_t site = 16 + 8 * l;

@@ -105,6 +105,7 @@ SIGNATURES = [
     ("gt_likelihood_euler", _c.c_int, [_c.c_void_p] + [_c.c_void_p] * 5 + [_c.c_int64, _c.c_int64, _c.c_int32] +
      [_c.c_void_p] * 2 + [_c.c_void_p, _c.c_size_t, _c.c_void_p]),
     ("gt_text_encoder_create", _c.c_int, [_c.c_int] * 9 + [_c.c_void_p]),
+    ("gt_text_encoder_create_buckets", _c.c_int, [_c.c_int] * 10 + [_c.c_void_p]),
     ("gt_text_encoder_destroy", None, [_c.c_void_p]),
     ("gt_text_encoder_num_params", _c.c_int, [_c.c_void_p]),
     ("gt_text_encoder_param_name", _c.c_char_p, [_c.c_void_p, _c.c_int]),

@@ -182,9 +182,10 @@ def estimator_flops(B: int, T: int, n_spks: int = 1) -> int:
 # ---- text encoder (model/text_encoder.py:285-335; GradTTS builds it speaker-agnostic, tts.py:49-51) ----------
 def text_encoder_param_shapes(n_vocab: int = 149, n_feats: int = 80, n_channels: int = 192,
                               filter_channels: int = 768, filter_channels_dp: int = 256, n_heads: int = 2,
-                              n_layers: int = 6, kernel_size: int = 3, window_size: int = 4):
+                              n_layers: int = 6, kernel_size: int = 3, window_size: int = 4, n_buckets=None):
     """state_dict keys and shapes of the reference TextEncoder, in its registration order (the order
-    tests/golden/gradtts_layout.json records from the real module, without the ``encoder.`` prefix)."""
+    tests/golden/gradtts_layout.json records from the real module, without the ``encoder.`` prefix); with ``n_buckets``
+    those of the bucket form."""
     C, kc = n_channels, n_channels // n_heads
     out = OrderedDict()
     out["emb.weight"] = (n_vocab, C)
@@ -198,23 +199,31 @@ def text_encoder_param_shapes(n_vocab: int = 149, n_feats: int = 80, n_channels:
     out["prenet.proj.bias"] = (C,)
     for l in range(n_layers):
         p = f"encoder.attn_layers.{l}."
-        out[p + "emb_rel_k"] = (1, 2 * window_size + 1, kc)
-        out[p + "emb_rel_v"] = (1, 2 * window_size + 1, kc)
+        if n_buckets:
+            out[p + "table"] = (n_buckets, n_heads)
+        else:
+            out[p + "emb_rel_k"] = (1, 2 * window_size + 1, kc)
+            out[p + "emb_rel_v"] = (1, 2 * window_size + 1, kc)
         for n in ("conv_q", "conv_k", "conv_v", "conv_o"):
             out[p + n + ".weight"] = (C, C, 1)
             out[p + n + ".bias"] = (C,)
-    for l in range(n_layers):
-        out[f"encoder.norm_layers_1.{l}.gamma"] = (C,)
-        out[f"encoder.norm_layers_1.{l}.beta"] = (C,)
+    if n_buckets:
+        out["encoder.norm_in.gamma"] = (C,)
+        out["encoder.norm_in.beta"] = (C,)
+    for key in (("norm_post_1", "norm_pre_1") if n_buckets else ("norm_layers_1",)):
+        for l in range(n_layers):
+            out[f"encoder.{key}.{l}.gamma"] = (C,)
+            out[f"encoder.{key}.{l}.beta"] = (C,)
     for l in range(n_layers):
         p = f"encoder.ffn_layers.{l}."
         out[p + "conv_1.weight"] = (filter_channels, C, kernel_size)
         out[p + "conv_1.bias"] = (filter_channels,)
         out[p + "conv_2.weight"] = (C, filter_channels, kernel_size)
         out[p + "conv_2.bias"] = (C,)
-    for l in range(n_layers):
-        out[f"encoder.norm_layers_2.{l}.gamma"] = (C,)
-        out[f"encoder.norm_layers_2.{l}.beta"] = (C,)
+    for key in (("norm_post_2", "norm_pre_2") if n_buckets else ("norm_layers_2",)):
+        for l in range(n_layers):
+            out[f"encoder.{key}.{l}.gamma"] = (C,)
+            out[f"encoder.{key}.{l}.beta"] = (C,)
     out["proj_m.weight"] = (n_feats, C, 1)
     out["proj_m.bias"] = (n_feats,)
     Fd = filter_channels_dp

@@ -60,7 +60,7 @@ class MultiHeadAttention(torch.nn.Module):
         super().__init__()
         if window_size is None or not heads_share or proximal_bias:
             raise ValueError("the HIP encoder implements the reference configuration: shared relative embeddings "
-                             "within a window, no proximal bias")
+                             "within a window, no proximal bias; n_buckets gives the bucket form")
         self.n_heads = n_heads
         self.window_size = window_size
         self.k_channels = channels // n_heads
@@ -71,6 +71,18 @@ class MultiHeadAttention(torch.nn.Module):
         self.emb_rel_k = torch.nn.Parameter(torch.randn(1, window_size * 2 + 1, self.k_channels) * rel_stddev)
         self.emb_rel_v = torch.nn.Parameter(torch.randn(1, window_size * 2 + 1, self.k_channels) * rel_stddev)
         self.conv_o = torch.nn.Conv1d(channels, out_channels, 1)
+
+
+class BucketAttention(torch.nn.Module):
+    """Self-attention of the encoder's bucket form (parameters only): one bias per bucket of distances and head."""
+
+    def __init__(self, channels, n_heads, n_buckets):
+        super().__init__()
+        self.table = torch.nn.Parameter(torch.randn(n_buckets, n_heads) * (channels // n_heads) ** -0.5)
+        self.conv_q = torch.nn.Conv1d(channels, channels, 1)
+        self.conv_k = torch.nn.Conv1d(channels, channels, 1)
+        self.conv_v = torch.nn.Conv1d(channels, channels, 1)
+        self.conv_o = torch.nn.Conv1d(channels, channels, 1)
 
 
 class FFN(torch.nn.Module):
@@ -101,10 +113,31 @@ class Encoder(torch.nn.Module):
             self.norm_layers_2.append(LayerNorm(hidden_channels))
 
 
+class BucketEncoder(torch.nn.Module):
+    """The layers of the bucket form (parameters only): h = norm_in(x), then for the attention and the FFN of each
+    layer x = x + norm_post(block(h)), h = norm_pre(x); the last h is the output."""
+
+    def __init__(self, hidden_channels, filter_channels, n_heads, n_layers, kernel_size, n_buckets, p_dropout=0.0):
+        super().__init__()
+        norms = lambda: torch.nn.ModuleList(LayerNorm(hidden_channels) for _ in range(n_layers))
+        self.attn_layers = torch.nn.ModuleList(BucketAttention(hidden_channels, n_heads, n_buckets)
+                                               for _ in range(n_layers))
+        self.norm_in = LayerNorm(hidden_channels)
+        self.norm_post_1, self.norm_pre_1 = norms(), norms()
+        self.ffn_layers = torch.nn.ModuleList(FFN(hidden_channels, hidden_channels, filter_channels, kernel_size,
+                                                  p_dropout=p_dropout) for _ in range(n_layers))
+        self.norm_post_2, self.norm_pre_2 = norms(), norms()
+
+
 class TextEncoder(torch.nn.Module):
     """``TextEncoder(n_vocab, n_feats, n_channels, filter_channels, filter_channels_dp, n_heads, n_layers,
-    kernel_size, p_dropout, window_size=None, spk_emb_dim=64, n_spks=1)``; ``forward(x, x_lengths, spk=None)`` ->
-    (mu [B, n_feats, Tx], logw [B, 1, Tx], x_mask [B, 1, Tx]).
+    kernel_size, p_dropout, window_size=None, spk_emb_dim=64, n_spks=1, n_buckets=None, max_distance=128)``;
+    ``forward(x, x_lengths, spk=None)`` -> (mu [B, n_feats, Tx], logw [B, 1, Tx], x_mask [B, 1, Tx]).
+
+    ``n_buckets`` (with ``window_size=None``) builds the bucket form: the layers attend with a learned bias per bucket
+    of distances (``gradtts_amd.attention.bucket_attention``) up to ``max_distance`` instead of relative embeddings
+    within a window, and their blocks are joined by ``gradtts_amd.norm.residual_norm`` steps. Heads may have any size
+    up to 128. Its training pass keeps no attention probabilities, so ``p_dropout`` does not fall on them.
 
     With gradients enabled and parameters that require them, or in train mode with p_dropout > 0, ``forward`` is the
     training pass
@@ -114,8 +147,11 @@ class TextEncoder(torch.nn.Module):
     from torch's CPU generator; in eval mode none do. Otherwise it is the inference pass (eval semantics)."""
 
     def __init__(self, n_vocab, n_feats, n_channels, filter_channels, filter_channels_dp, n_heads, n_layers,
-                 kernel_size, p_dropout, window_size=None, spk_emb_dim=64, n_spks=1):
+                 kernel_size, p_dropout, window_size=None, spk_emb_dim=64, n_spks=1, n_buckets=None, max_distance=128):
         super().__init__()
+        if n_buckets is not None and window_size is not None:
+            raise ValueError("window_size and n_buckets exclude each other: relative embeddings within a window, or a "
+                             "bias by buckets of distances")
         if n_spks > 1:
             raise ValueError("GradTTS builds its TextEncoder speaker-agnostic (tts.py:49-51); n_spks > 1 is not "
                              "implemented")
@@ -126,8 +162,13 @@ class TextEncoder(torch.nn.Module):
         self.emb = torch.nn.Embedding(n_vocab, n_channels)
         torch.nn.init.normal_(self.emb.weight, 0.0, n_channels ** -0.5)
         self.prenet = ConvReluNorm(n_channels, n_channels, n_channels, kernel_size=5, n_layers=3, p_dropout=0.5)
-        self.encoder = Encoder(n_channels, filter_channels, n_heads, n_layers, kernel_size, p_dropout,
-                               window_size=window_size)
+        self.n_buckets, self.max_distance = n_buckets, max_distance
+        if n_buckets is None:
+            self.encoder = Encoder(n_channels, filter_channels, n_heads, n_layers, kernel_size, p_dropout,
+                                   window_size=window_size)
+        else:
+            self.encoder = BucketEncoder(n_channels, filter_channels, n_heads, n_layers, kernel_size, n_buckets,
+                                         p_dropout)
         self.proj_m = torch.nn.Conv1d(n_channels, n_feats, 1)
         self.proj_w = DurationPredictor(n_channels, filter_channels_dp, kernel_size, p_dropout)
         self._handle = None
@@ -137,9 +178,13 @@ class TextEncoder(torch.nn.Module):
         L = lib()
         if self._handle is None:
             h = ctypes.c_void_p()
-            check(L.gt_text_encoder_create(self.n_vocab, self.n_feats, self.n_channels, self.filter_channels,
-                                           self.filter_channels_dp, self.n_heads, self.n_layers, self.kernel_size,
-                                           self.window_size, ctypes.byref(h)), "gt_text_encoder_create")
+            sizes = (self.n_vocab, self.n_feats, self.n_channels, self.filter_channels, self.filter_channels_dp,
+                     self.n_heads, self.n_layers, self.kernel_size)
+            if self.n_buckets is None:
+                check(L.gt_text_encoder_create(*sizes, self.window_size, ctypes.byref(h)), "gt_text_encoder_create")
+            else:
+                check(L.gt_text_encoder_create_buckets(*sizes, self.n_buckets, self.max_distance, ctypes.byref(h)),
+                      "gt_text_encoder_create_buckets")
             self._handle = h
         sig = tuple((p.data_ptr(), p._version) for p in self.parameters())
         if sig != self._synced:

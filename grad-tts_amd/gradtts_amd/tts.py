@@ -2,7 +2,8 @@
 ``grad_*.pt`` loads unchanged), ``forward`` = text -> encoder -> durations / alignment -> decoder entirely on the
 MI355X (gradtts_amd.text_encoder + gradtts_amd.diffusion), ``compute_loss`` = the reference's training objective
 (encoder training pass, log-prior + MAS, duration loss, ``out_size`` crop, ``mu_y``, diffusion loss, prior loss) with
-every gradient computed by the library, ``get_score_model`` for likelihood rescoring."""
+every gradient computed by the library, ``get_score_model`` for likelihood rescoring. ``n_buckets`` and
+``max_distance`` (with ``window_size=None``) give its text encoder the bucket form."""
 import random
 
 import torch
@@ -14,7 +15,7 @@ from .text_encoder import TextEncoder, align_durations
 class GradTTS(torch.nn.Module):
     def __init__(self, n_vocab, n_spks, spk_emb_dim, n_enc_channels, filter_channels, filter_channels_dp, n_heads,
                  n_enc_layers, enc_kernel, enc_dropout, window_size, n_feats, dec_dim, beta_min, beta_max, pe_scale,
-                 compute_dtype=torch.float32):
+                 compute_dtype=torch.float32, n_buckets=None, max_distance=128):
         super().__init__()
         self.n_vocab = n_vocab
         self.n_spks = n_spks
@@ -26,7 +27,8 @@ class GradTTS(torch.nn.Module):
         elif n_spks > 1:
             self.spk_emb = torch.nn.Embedding(n_spks, spk_emb_dim)
         self.encoder = TextEncoder(n_vocab, n_feats, n_enc_channels, filter_channels, filter_channels_dp, n_heads,
-                                   n_enc_layers, enc_kernel, enc_dropout, window_size)
+                                   n_enc_layers, enc_kernel, enc_dropout, window_size, n_buckets=n_buckets,
+                                   max_distance=max_distance)
         self.decoder = Diffusion(n_feats, dec_dim, n_spks, spk_emb_dim, beta_min, beta_max, pe_scale,
                                  compute_dtype=compute_dtype)
 

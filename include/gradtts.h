@@ -214,6 +214,17 @@ int gt_likelihood_euler(gt_decoder* dec, const float* data, const float* mask, c
 typedef struct gt_text_encoder gt_text_encoder;
 int gt_text_encoder_create(int n_vocab, int n_feats, int n_channels, int filter_channels, int filter_channels_dp,
                            int n_heads, int n_layers, int kernel_size, int window_size, gt_text_encoder** out);
+/* The encoder's bucket form: the layers' attention is gt_bucket_attention (bidirectional, all heads, one table
+ * "encoder.attn_layers.<l>.table" [n_buckets][n_heads] a layer) in place of the windowed relative embeddings, and its
+ * blocks are joined by gt_residual_norm steps: h = N_in(x), then for the attention and the FFN of each layer
+ * x += N_post(block(h)), h = N_pre(x), parameters "encoder.norm_in", "encoder.norm_post_1.<l>", "norm_pre_1",
+ * "norm_post_2", "norm_pre_2" (.gamma, .beta); the encoder's output is the last h. Prenet, projections, duration
+ * predictor and every function below are the same. Its training pass keeps no [Tx,Tx] tensor; p_dropout falls on the
+ * blocks' outputs and the FFN's hidden channels, not on the attention's probabilities. n_heads must divide n_channels
+ * <= 256, heads <= 128 channels, kernel_size odd; n_buckets, max_distance as gt_bucket_attention. */
+int gt_text_encoder_create_buckets(int n_vocab, int n_feats, int n_channels, int filter_channels,
+                                   int filter_channels_dp, int n_heads, int n_layers, int kernel_size, int n_buckets,
+                                   int max_distance, gt_text_encoder** out);
 void gt_text_encoder_destroy(gt_text_encoder* enc);
 int gt_text_encoder_num_params(gt_text_encoder* enc);
 const char* gt_text_encoder_param_name(gt_text_encoder* enc, int i);
@@ -363,8 +374,8 @@ int gt_bucket_attention_backward(const gt_bucket_attention* a, const void* out, 
  *   out = x + scale gate N1(y),  h = N2(out),  N(t) = u w + b over the C channels,
  *   u = (t - mean) / sqrt(var + eps), or t / sqrt(mean(t^2) + eps) with rms = 1;
  * x, y, out, h [B,T,C] contiguous of one element type; gate [C], or [B,C] with gate_per_batch, or NULL (1); weights
- * and biases [C] (biases may be NULL); all parameters fp32. C <= 8192. lengths [B]: rows t >= lengths[b] are not read,
- * their outputs and gradients are zero (NULL: all of T). stats: NULL, or [B,T,4] fp32 for the backward.
+ * and biases [C] (biases may be NULL); all parameters fp32. C <= 8192, B <= 65535. lengths [B]: rows t >= lengths[b]
+ * are not read, their outputs and gradients are zero (NULL: all of T). stats: NULL, or [B,T,4] fp32 for the backward.
  * backward: from the forward's arguments, its stats, dout and dh: dx, dy [B,T,C] and the parameters' fp32 gradients
  * (those of absent parameters must be NULL; dgate has the gate's shape). Fixed summation order. */
 typedef struct {

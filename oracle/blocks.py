@@ -174,3 +174,45 @@ def residual_norm(x, y, post_weight, pre_weight, post_bias=None, pre_bias=None, 
         cols("dgate", scale * d * n1, abs(scale) * (ed * ((u1 * w1).abs() + b1.abs()) + d.abs() * en1 +
                                                     n * U32 * d.abs() * ((u1 * w1).abs() + b1.abs())), gate.dim() == 2)
     return val, err
+
+
+def bucket_text_encoder(p, tokens, x_lengths, n_layers, n_heads, max_distance, drop=None):
+    """The text encoder's bucket form in the parameters' type, by autograd's operations: prenet, projections and
+    duration predictor as oracle.text_encoder, layers h = N_in(x); x += N_post(block(h)), h = N_pre(x). drop: None, or
+    oracle.text_encoder.Dropouts (its masks fall on the blocks' outputs and the FFN's hidden channels)."""
+    from .text_encoder import conv, ln
+    D = (lambda site, v, q: drop.chan(site, v, q)) if drop is not None else (lambda site, v, q: v)
+    pe, pp = (drop.p, drop.pp) if drop is not None else (0.0, 0.0)
+    C = p["emb.weight"].shape[1]
+    x = (p["emb.weight"][tokens] * math.sqrt(C)).transpose(1, -1)
+    T = x.shape[2]
+    live = torch.arange(T)[None] < x_lengths[:, None]
+    m = live.unsqueeze(1).to(x.dtype)
+    x_org = x
+    for i in range(3):
+        x = conv(p, f"prenet.conv_layers.{i}", x * m)
+        x = D(1 + i, torch.relu(ln(p, f"prenet.norm_layers.{i}", x)), pp)
+    x = (x_org + conv(p, "prenet.proj", x)) * m
+    nb = p["encoder.attn_layers.0.table"].shape[0]
+    near = {o: bucket(o, nb, False, max_distance) for o in range(-T, T + 1)}
+    idx = torch.tensor([[near[j - i] for j in range(T)] for i in range(T)])
+    shut = torch.where(live[:, None, None, :], 0.0, -1e30).to(x.dtype)   # a row without keys is masked afterwards
+    h = ln(p, "encoder.norm_in", x) * m
+    heads = lambda t: t.reshape(len(t), n_heads, C // n_heads, T).transpose(2, 3)
+    for l in range(n_layers):
+        a, f, site = f"encoder.attn_layers.{l}.", f"encoder.ffn_layers.{l}.", 16 + 8 * l
+        q, k, v = (heads(conv(p, a + n, h)) for n in ("conv_q", "conv_k", "conv_v"))
+        s = torch.matmul(q, k.transpose(2, 3)) * (C // n_heads) ** -0.5 + p[a + "table"][idx].permute(2, 0, 1)[None]
+        y = torch.matmul(torch.softmax(s + shut, -1), v).transpose(2, 3).reshape(x.shape) * m
+        y = D(site + 1, conv(p, a + "conv_o", y), pe)
+        x = (x + ln(p, f"encoder.norm_post_1.{l}", y)) * m
+        h = ln(p, f"encoder.norm_pre_1.{l}", x) * m
+        y = D(site + 2, torch.relu(conv(p, f + "conv_1", h)), pe)
+        y = D(site + 3, conv(p, f + "conv_2", y * m) * m, pe)
+        x = (x + ln(p, f"encoder.norm_post_2.{l}", y)) * m
+        h = ln(p, f"encoder.norm_pre_2.{l}", x) * m
+    mu = conv(p, "proj_m", h) * m
+    h = h.detach()
+    d = D(8, ln(p, "proj_w.norm_1", torch.relu(conv(p, "proj_w.conv_1", h * m))), pe)
+    d = D(9, ln(p, "proj_w.norm_2", torch.relu(conv(p, "proj_w.conv_2", d * m))), pe)
+    return mu, conv(p, "proj_w.proj", d * m) * m, m
