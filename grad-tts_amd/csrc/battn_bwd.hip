@@ -34,6 +34,12 @@ GT_DEV float diagonals(const float (&x)[16]) {
   return a;
 }
 
+// fp16 rounds P <= 1 below 2^-14 to steps of 2^-25: a row of thousands of keys loses digits of it. There dK dV forms
+// 2^15 P, in the exponent, and takes the factor out of dV's sums and, by way of delta (kept times 2^-15) and one FMA in
+// place of a subtraction, of dS. The other types have fp32's range.
+template <class T> constexpr float kUp = std::is_same<T, f16>::value ? 15.f : 0.f;
+template <class T> constexpr float kDown = std::is_same<T, f16>::value ? 0x1p-15f : 1.f;
+
 // ================================================================ dQ, delta, table partials
 // The product o . do with the rounded o, formed from rounded P, is off by about u |o| |do| (u = half a step of the
 // type), which weighs when few keys share a row: dS = P (dP - delta) is then a small difference. Rows whose keys all lie
@@ -222,7 +228,7 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 2 || sizeof(T) == 4 ? 1 : 2) voi
     step(t, std::integral_constant<int, 0>());
     if (t + 1 < ntile) step(t + 1, std::integral_constant<int, 1>());
   }
-  if (qi < p.Tq && hh == 0 && ws == 0) p.delta[srow] = in ? delta : 0.f;
+  if (qi < p.Tq && hh == 0 && ws == 0) p.delta[srow] = in ? delta * kDown<T> : 0.f;
   if constexpr (WS == 1) {
     if (qi < p.Tq) {
       T* qo = (T*)p.dq + b * p.dqs.b + h * p.dqs.h + (long)qi * p.dqs.t;
@@ -345,7 +351,8 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 2 || sizeof(T) == 4 || DP > 64 ?
         __syncthreads();   // the last head's tiles and bias are done with
         if (SH::NBUF == 2) load(0);
         build_ext<T>(p, h, 1, h, ext0, tid, NT);
-        const float blo = table_at<T>(p, p.side - 1, h) * kLog2e, bhi = p.causal ? 0.f : table_at<T>(p, 2 * p.side - 1, h) * kLog2e;
+        const float blo = table_at<T>(p, p.side - 1, h) * kLog2e + kUp<T>;
+        const float bhi = p.causal ? 0.f : table_at<T>(p, 2 * p.side - 1, h) * kLog2e + kUp<T>;
         auto step = [&](int t, auto buf) {   // buf: t & 1, a constant at both calls
           if constexpr (SH::NBUF == 2) {
             lds_ready();
@@ -364,7 +371,7 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 2 || sizeof(T) == 4 || DP > 64 ?
             if (p.causal && pmax < wk0) continue;
             const int dmax = wk0 + 31 - pmin, dmin = wk0 - pmax;
             f32x16 s, dp;
-            float off = 0.f;
+            float off = kUp<T>;
             constexpr int CH = KS % 4 ? 3 : 4;
             frag a[CH], c[CH];
             auto read = [&](int x0) {
@@ -402,7 +409,7 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 2 || sizeof(T) == 4 || DP > 64 ?
               for (int e = 0; e < 4; ++e) {
                 const int j = 4 * jg + e;
                 pr[j] = expo<T>(s[j], p.c, off, ls[e]);
-                ds[j] = pr[j] * (dp[j] - de[e]);
+                ds[j] = pr[j] * (kDown<T> == 1.f ? dp[j] - de[e] : __builtin_fmaf(dp[j], kDown<T>, -de[e]));
               }
             }
             if (wk0 + 31 >= klen || qq + 31 >= qlen || (p.causal && dmax > 0)) {
@@ -451,14 +458,14 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 2 || sizeof(T) == 4 || DP > 64 ?
       } else if (p.gsplit > 1) {
         if (in) {
           store_rows<float, DP>(part(ki), dk, p.scale, D, v4, hh);
-          store_rows<float, DP>(part(ki) + half, dv, 1.f, D, v4, hh);
+          store_rows<float, DP>(part(ki) + half, dv, kDown<T>, D, v4, hh);
         } else {
           zero_rows<float, DP>(part(ki), D, v4, hh);
           zero_rows<float, DP>(part(ki) + half, D, v4, hh);
         }
       } else if (in) {
         store_rows<T, DP>(ko + (long)ki * p.dks.t, dk, p.scale, D, p.vec, hh);
-        store_rows<T, DP>(vo + (long)ki * p.dvs.t, dv, 1.f, D, p.vec, hh);
+        store_rows<T, DP>(vo + (long)ki * p.dvs.t, dv, kDown<T>, D, p.vec, hh);
       } else {
         zero_rows<T, DP>(ko + (long)ki * p.dks.t, D, p.vec, hh);
         zero_rows<T, DP>(vo + (long)ki * p.dvs.t, D, p.vec, hh);
@@ -470,7 +477,7 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 2 || sizeof(T) == 4 || DP > 64 ?
         if (p.gsplit > 1) store4_row(part(wk0 + row), d, x, D, v4);
         else store4_row(ko + (long)(wk0 + row) * p.dks.t, d, x, D, p.vec);
       });
-      join<DP, WS>(smem, dv, 1.f, wr, ws, lane, [&](int row, int d, float* x) {
+      join<DP, WS>(smem, dv, kDown<T>, wr, ws, lane, [&](int row, int d, float* x) {
         if (wk0 + row >= p.Tk) return;
         if (wk0 + row >= klen) x[0] = x[1] = x[2] = x[3] = 0.f;
         if (p.gsplit > 1) store4_row(part(wk0 + row) + half, d, x, D, v4);
