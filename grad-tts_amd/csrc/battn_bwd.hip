@@ -118,8 +118,9 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 2 || sizeof(T) == 4 ? 1 : 2) voi
     const int dmax = kk + 31 - pmin, dmin = kk - pmax;
     f32x16 s;
     float off = 0.f;
-    // four fragments of each operand at a time: read together, then multiplied
-    constexpr int CH = KS % 4 ? 3 : 4;
+    // fragments of each operand read together, then multiplied: four, at 128 channels two (their registers spilled
+    // there: 111 us against 96 for 2 x 16 heads, 2048 causal rows)
+    constexpr int CH = KS % 4 ? 3 : KS > 4 ? 2 : 4;
     frag a[CH], c[CH];
     auto read = [&](int k0) {
 #pragma unroll
@@ -520,21 +521,33 @@ template <class T, int N> __global__ __launch_bounds__(256) void ba_gsum_kernel(
 // every other CU idle (not where the spread form's LDS would not hold the table sums of far borders). dK dV first splits the
 // heads of a group.
 constexpr int kSat = 4 * 32 * 4;   // bytes of `sat`, four waves
-struct BwdPlan { int rows_q, rows_k, gsplit, ntq, ntk, ranks_k; };
-int rows_of(const BaParams& p, long heads, int T) {
-  const int halves = p.causal ? 2 : 1;   // (a causal workgroup is half as long, or two tiles)
-  return heads * ((T + 127) / 128) >= 512 * halves ? 128 : heads * ((T + 63) / 64) >= 128 * halves ? 64 : 32;
+struct BwdPlan { int rows_q, rows_k, gsplit, ntq, ntk, ranks_k, pair_k; };
+// Rows a workgroup, by how many workgroups that makes; us of the backward with 32 / 64 / 128 rows at (heads x batch, T,
+// head size):
+//   128 rows from two workgroups a CU on (fp32, not causal: one): bf16 (128, 512, 64) 148 / 84 / 67, causal 124 / 67 / 61,
+//   below (64, 512, 64) 80 / 49 / 51; fp32 (64, 512, 128) 790 / 458 / 364; but not the 16-bit dQ of 128 channels, whose
+//   registers spill there (2 x 16 causal heads, 2048 rows: dQ 97 us with 64, 116 with 128);
+//   64 rows from 192 workgroups on: bf16 (64, 190, 64) 39 / 30, fp32 86 / 58; below (32, 190, 64) 28 / 30, 47 / 57. fp32
+//   of more than 64 channels, one workgroup a CU either way: always (32, 190, 128) 118 / 101, (8, 64, 96) 52 / 46.
+int rows_of(const BaParams& p, int dtype, long heads, int T) {
+  const bool wide = dtype == 0;
+  if (heads * ((T + 127) / 128) >= (wide && !p.causal ? 256 : 512)) return 128;
+  return heads * ((T + 63) / 64) >= 192 || (wide && p.D > 64) ? 64 : 32;
 }
-BwdPlan plan_bwd(const BaParams& p) {
+BwdPlan plan_bwd(const BaParams& p, int dtype) {
   BwdPlan b;
   const int dp = p.D <= 64 ? 64 : p.D <= 96 ? 96 : 128, spread = 1024 * dp;   // the spread Shape's bytes, any type
-  b.rows_q = rows_of(p, (long)p.B * p.Hq, p.Tq);
+  b.rows_q = rows_of(p, dtype, (long)p.B * p.Hq, p.Tq);
+  if (b.rows_q == 128 && dtype != 0 && dp == 128) b.rows_q = 64;
   if (b.rows_q == 32 && spread + 5 * host_ext_bytes(p) + kSat > kLds) b.rows_q = 64;
   b.ntq = (p.Tq + b.rows_q - 1) / b.rows_q;
   const long kv = (long)p.B * p.Hkv;
-  b.rows_k = rows_of(p, kv * p.G, p.Tk);
+  b.rows_k = rows_of(p, dtype, kv * p.G, p.Tk);
   b.ntk = (p.Tk + b.rows_k - 1) / b.rows_k;
-  b.ranks_k = p.causal ? (b.ntk + 1) / 2 : b.ntk;   // paired
+  // causal dK dV: a tile and its mirror image a workgroup, so that all are equally long, unless every tile has a CU of its
+  // own: bf16 (32, 2048, 128) 212 us paired, 271 not; (64, 190, 128) 51 and 41
+  b.pair_k = p.causal && kv * p.G * b.ntk > 256;
+  b.ranks_k = b.pair_k ? (b.ntk + 1) / 2 : b.ntk;
   b.gsplit = 1;
   while (b.gsplit < p.G && kv * b.ranks_k * b.gsplit < 256)
     do ++b.gsplit; while (p.G % b.gsplit);
@@ -552,7 +565,7 @@ template <class T, int DP, int WR> hipError_t bwd_k(BaParams p, const BwdPlan& b
   typedef Shape<T, DP, WR, 4 / WR> SH;
   const long grid = (long)p.B * p.Hkv * b.gsplit * b.ranks_k;
   p.ntile = b.ntk;
-  p.pair = p.causal;
+  p.pair = b.pair_k;
   return launch(ba_dkv_kernel<T, DP, WR, 4 / WR>, grid, 256, SH::BYTES + SH::NBUF * 2 * SH::KT * 4 + host_ext_bytes(p), p, s);
 }
 template <class T, int DP> hipError_t bwd(const BaParams& p, const BwdPlan& b, hipStream_t s) {
@@ -581,12 +594,12 @@ size_t table_bytes(const BaParams& p, const BwdPlan& b) { return up256((size_t)p
 
 }  // namespace
 
-size_t ba_backward_ws(const BaParams& p, int) {
-  const BwdPlan b = plan_bwd(p);
+size_t ba_backward_ws(const BaParams& p, int dtype) {
+  const BwdPlan b = plan_bwd(p, dtype);
   return delta_bytes(p) + table_bytes(p, b) + (b.gsplit > 1 ? (size_t)2 * b.gsplit * p.B * p.Tk * p.Hkv * p.D * 4 : 0) + 256;
 }
 hipError_t launch_ba_backward(BaParams p, int dtype, void* ws, hipStream_t s) {
-  const BwdPlan b = plan_bwd(p);
+  const BwdPlan b = plan_bwd(p, dtype);
   char* w = align256(ws);
   p.delta = (float*)w;
   p.tpart = (float*)(w + delta_bytes(p));

@@ -430,12 +430,18 @@ template <class T> __global__ __launch_bounds__(256) void ba_join_kernel(BaParam
 }
 
 // ---------------------------------------------------------------- launches
-// Shared tiles of 128 rows, or of 64 where that leaves fewer than two workgroups a CU, as long as these give every CU
-// one; else spread rows: blocks of 32, and, where few blocks meet long caches, key ranges with workgroups of their own
-// (about four a CU, of 512 keys at least), joined afterwards.
+// Rows a workgroup, by how many workgroups that makes; us for spread / 64 / 128 rows at (heads x batch, T, head size):
+//   128 rows from two workgroups a CU on (fp32, whose products outlast the copies: one): bf16 (128, 512, 64) 30 / 25 / 19,
+//   below (64, 512, 128) 30 / 22 / 23, causal (64, 512, 64) 16 / 16 / 19; fp32 (64, 512, 128) 134 / 121 / 100;
+//   64 rows from 192 workgroups on: bf16 (64, 512, 64) 18 / 15, fp32 (64, 190, 64) 20 / 17; below: fp32 (32, 190, 64)
+//   12 / 16, bf16 causal (64, 190, 128) 12 / 18;
+//   else spread rows, blocks of 32. Where these are fewer than the CUs and the cache is longer than 1024 keys, key ranges of
+//   256 keys at least have workgroups of their own, one a CU in all, and are joined afterwards: one query of 16 bf16 heads
+//   over 8192 keys 69 us alone, 16 split; 2 fp32 heads over 700 keys 12 alone, 13 split; over 2000 21 and 13. One range a
+//   CU, not four: 32 sequences of 8192 keys 108 us against 117, one of 65536 55 against 69.
 enum Form { SHARED4, SHARED2, SPREAD };
 struct FwdPlan { Form form; long units; };
-FwdPlan plan_fwd(BaParams& p) {
+FwdPlan plan_fwd(BaParams& p, int dtype) {
   p.nsplit = 1;
   const long heads = (long)p.B * p.Hq;
   auto groups = [&](int rows) {
@@ -444,8 +450,8 @@ FwdPlan plan_fwd(BaParams& p) {
     return heads * (p.pair ? (p.ntile + 1) / 2 : p.ntile);
   };
   if (p.Tq > 32) {
-    if (groups(128) >= 512) return {SHARED4, groups(128)};
-    if (groups(64) >= 128) return {SHARED2, groups(64)};
+    if (groups(128) >= (dtype == 0 ? 256 : 512)) return {SHARED4, groups(128)};
+    if (groups(64) >= 192) return {SHARED2, groups(64)};
   }
   FwdPlan f{SPREAD, 0};
   p.pair = 0;
@@ -456,11 +462,10 @@ FwdPlan plan_fwd(BaParams& p) {
   f.units = (long)p.B * p.Hkv * ((p.G + p.gp - 1) / p.gp) * p.ntile;
   constexpr int KT = 32 * WSP;
   p.split_keys = (p.Tk + KT - 1) / KT * KT;
-  if (f.units && f.units < 256 && p.Tk > 4 * KT) {
-    long n = (1024 + f.units - 1) / f.units;
-    if (n > 512) n = 512;
+  if (f.units && f.units < 256 && p.Tk > 8 * KT) {
+    const long n = (256 + f.units - 1) / f.units;
     long keys = ((p.Tk + n - 1) / n + KT - 1) / KT * KT;
-    if (keys < 4 * KT) keys = 4 * KT;
+    if (keys < 2 * KT) keys = 2 * KT;
     p.split_keys = (int)keys;
     p.nsplit = (int)((p.Tk + keys - 1) / keys);
   }
@@ -491,14 +496,14 @@ template <class T> hipError_t fwd_t(const BaParams& p, const FwdPlan& f, hipStre
 
 }  // namespace
 
-size_t ba_forward_ws(const BaParams& p0, int) {
+size_t ba_forward_ws(const BaParams& p0, int dtype) {
   BaParams p = p0;
-  const FwdPlan f = plan_fwd(p);
+  const FwdPlan f = plan_fwd(p, dtype);
   if (p.nsplit == 1) return 0;
   return up256((size_t)f.units * p.nsplit * 32 * p.D * 4) + (size_t)f.units * p.nsplit * 64 * 4 + 256;
 }
 hipError_t launch_ba_forward(BaParams p, int dtype, void* ws, hipStream_t s) {
-  const FwdPlan f = plan_fwd(p);
+  const FwdPlan f = plan_fwd(p, dtype);
   if (p.nsplit > 1) {
     char* w = align256(ws);
     p.part = (float*)w;

@@ -37,6 +37,10 @@ FORMS = [
     (4, 190, 190, 16, 4, 72, True, 32, 128, [190, 65, 64, 1], [190, 65, 64, 1], None),
     (4, 130, 150, 16, 8, 104, False, 32, 128, None, None, [20, 0, 0, -30]),
     (4, 130, 130, 16, 16, 33, True, 32, 128, None, None, None),
+    (6, 190, 190, 16, 16, 72, True, 32, 128, [190, 65, 64, 1, 0, 129], None, None),
+    (7, 150, 150, 16, 8, 24, True, 32, 128, None, [150, 1, 64, 65, 0, 128, 150], None),
+    (6, 140, 140, 16, 16, 109, True, 32, 128, None, None, None),
+    (6, 400, 400, 16, 4, 40, True, 32, 128, None, None, None),
     (1, 1, 5000, 8, 2, 128, True, 32, 128, None, None, [4999]),
     (3, 2, 1500, 4, 2, 64, True, 32, 128, [1500, 3, 0], None, [1498, 1, 0]),
     (2, 7, 1300, 6, 1, 50, False, 32, 128, [1300, 700], None, [300, 0]),
