@@ -4,6 +4,11 @@
 // Two kernels, each the sole writer of its rows, so that every sum has one order: dQ (with delta and the table's
 // partial sums) streams keys past 32-row query blocks, dK dV streams queries past key blocks. Scores and dP are formed
 // in both: 7 products instead of 5, against atomics or a T x T matrix in memory.
+//
+// Bound by the waves' own latency: at 128 channels the stationary rows, their sums and a block's fragments fill the
+// registers of one wave a SIMD (dK dV) or two (dQ), so products wait for LDS reads and exponentials more than they
+// overlap with them. 2 x 16 bf16 heads (4 key / value heads) of 2048 causal rows, 128 channels: dQ 96 us (0.54 PFLOP/s),
+// dK dV 117 (0.59), sums of head groups 14 (4.8 TB/s), table 5; 3 x 6 fp16 heads of a ragged 777, 80 channels: 40, 36, -, 4.
 #include <type_traits>
 
 #include "battn_core.h"
@@ -531,7 +536,7 @@ struct BwdPlan { int rows_q, rows_k, gsplit, ntq, ntk, ranks_k, pair_k; };
 //   of more than 64 channels, one workgroup a CU either way: always (32, 190, 128) 118 / 101, (8, 64, 96) 52 / 46.
 int rows_of(const BaParams& p, int dtype, long heads, int T) {
   const bool wide = dtype == 0;
-  if (heads * ((T + 127) / 128) >= (wide && !p.causal ? 256 : 512)) return 128;
+  if (fills128(dtype, T) && heads * ((T + 127) / 128) >= (wide && !p.causal ? 256 : 512)) return 128;
   return heads * ((T + 63) / 64) >= 192 || (wide && p.D > 64) ? 64 : 32;
 }
 BwdPlan plan_bwd(const BaParams& p, int dtype) {

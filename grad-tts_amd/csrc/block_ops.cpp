@@ -1,5 +1,5 @@
-// C ABI of the transformer-block operators (include/gradtts.h): argument checks and parameter blocks for battn.hip
-// and rnorm.hip.
+// C ABI of the transformer-block operators (include/gradtts.h): argument checks and parameter blocks for
+// battn_fwd.hip, battn_bwd.hip and rnorm.hip.
 #include <hip/hip_runtime.h>
 
 #include <cmath>

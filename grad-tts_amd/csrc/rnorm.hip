@@ -5,7 +5,10 @@
 // Bound by memory: the forward reads x and y and writes out and h once, the backward reads x, y, d out, dh and writes
 // dx and dy. One group of TPR threads holds a whole row in registers (E channels a thread), so both norms are two-pass
 // (mean, then centred squares) without reading anything twice; groups walk their rows with the next row's loads in
-// flight and with gate and weights, the same for every row of a batch entry, in registers.
+// flight and with gate and weights, the same for every row of a batch entry, in registers. bf16, where a copy reaches
+// 4.9 TB/s: forward, 4 x 4096 rows of 4096 (537 MB) in 117 us, 4.6 TB/s; backward, 4 x 2048 rows of 2048 (201 MB) in
+// 57 us, 3.6 TB/s (156 registers: three waves a SIMD), and 10 us for the column sums. Two rows' loads in flight instead
+// of one: the same times.
 #include "rnorm.h"
 
 #include "common.h"

@@ -1,9 +1,10 @@
-"""Attention with a learned relative position bias by buckets (csrc/battn.hip), with all gradients.
+"""Attention with a learned relative position bias by buckets (csrc/battn_fwd.hip, csrc/battn_bwd.hip), with all
+gradients.
 
 The text encoder's own attention (``text_encoder.MultiHeadAttention``) learns an embedding for each offset within a
 window of a few tokens and treats everything beyond alike; here every offset has a learned bias for each head, one for
 each small distance and one for each of some logarithmically wider ranges up to ``max_distance``, the last for all
-beyond.
+beyond. ``text_encoder.TextEncoder(n_buckets=...)`` is built on it.
 """
 from __future__ import annotations
 

@@ -1,6 +1,7 @@
 """The residual step between two blocks of a transformer with norms on both sides of a block (csrc/rnorm.hip): the
 norm after the finished block, its gate and residual scale, the residual sum and the norm before the next block in one
-pass, with all gradients. The text encoder's own residual steps are ``LayerNorm(x + y)`` (``text_encoder.Encoder``).
+pass, with all gradients. The text encoder's own residual steps are ``LayerNorm(x + y)`` (``text_encoder.Encoder``); its bucket form
+(``text_encoder.BucketEncoder``) takes this one.
 """
 from __future__ import annotations
 
