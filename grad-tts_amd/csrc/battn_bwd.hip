@@ -522,9 +522,6 @@ template <class T, int N> __global__ __launch_bounds__(256) void ba_gsum_kernel(
 }
 
 // ---------------------------------------------------------------- launches
-// Rows of a workgroup: 128, or 64 where that leaves fewer than two workgroups' work a CU, or 32 (spread) where 64 leave
-// every other CU idle (not where the spread form's LDS would not hold the table sums of far borders). dK dV first splits the
-// heads of a group.
 constexpr int kSat = 4 * 32 * 4;   // bytes of `sat`, four waves
 struct BwdPlan { int rows_q, rows_k, gsplit, ntq, ntk, ranks_k, pair_k; };
 // Rows a workgroup, by how many workgroups that makes; us of the backward with 32 / 64 / 128 rows at (heads x batch, T,
@@ -544,6 +541,7 @@ BwdPlan plan_bwd(const BaParams& p, int dtype) {
   const int dp = p.D <= 64 ? 64 : p.D <= 96 ? 96 : 128, spread = 1024 * dp;   // the spread Shape's bytes, any type
   b.rows_q = rows_of(p, dtype, (long)p.B * p.Hq, p.Tq);
   if (b.rows_q == 128 && dtype != 0 && dp == 128) b.rows_q = 64;
+  // (the spread form's LDS does not hold the table sums of far borders)
   if (b.rows_q == 32 && spread + 5 * host_ext_bytes(p) + kSat > kLds) b.rows_q = 64;
   b.ntq = (p.Tq + b.rows_q - 1) / b.rows_q;
   const long kv = (long)p.B * p.Hkv;
@@ -553,6 +551,7 @@ BwdPlan plan_bwd(const BaParams& p, int dtype) {
   // own: bf16 (32, 2048, 128) 212 us paired, 271 not; (64, 190, 128) 51 and 41
   b.pair_k = p.causal && kv * p.G * b.ntk > 256;
   b.ranks_k = b.pair_k ? (b.ntk + 1) / 2 : b.ntk;
+  // the heads of a group in several workgroups until every CU has one
   b.gsplit = 1;
   while (b.gsplit < p.G && kv * b.ranks_k * b.gsplit < 256)
     do ++b.gsplit; while (p.G % b.gsplit);

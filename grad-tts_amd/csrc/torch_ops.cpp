@@ -22,8 +22,11 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
+
+#include <unordered_set>
 
 #include "gradtts.h"
 
@@ -430,14 +433,30 @@ void check_capture(std::initializer_list<const at::Tensor*> inputs) {
   const auto cur = c10::hip::getCurrentHIPStream(first.device().index());
   hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
   if (hipStreamIsCapturing(cur.stream(), &st) != hipSuccess || st == hipStreamCaptureStatusNone) return;
-  for (const at::Tensor* t : inputs) {
-    if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
-    const auto acc = torch::autograd::impl::try_get_grad_accumulator(*t);
-    if (!acc) continue;
+  auto check = [&](torch::autograd::Node* acc) {
     const auto s = acc->stream();
     TORCH_CHECK(!s.has_value() || *s == cur.unwrap(),
                 "gradtts: a graph capture with gradients while an eager autograd graph of the same parameters is alive "
                 "(its gradient accumulators run on another stream); free that graph (its loss and outputs) first");
+  };
+  // the inputs that are leaves, and the leaves that the others were made from
+  std::vector<torch::autograd::Node*> todo;
+  std::unordered_set<torch::autograd::Node*> seen;
+  for (const at::Tensor* t : inputs) {
+    if (!t->defined() || !t->requires_grad()) continue;
+    if (t->is_leaf()) {
+      if (const auto acc = torch::autograd::impl::try_get_grad_accumulator(*t)) check(acc.get());
+    } else if (t->grad_fn()) {
+      todo.push_back(t->grad_fn().get());
+    }
+  }
+  while (!todo.empty()) {
+    torch::autograd::Node* n = todo.back();
+    todo.pop_back();
+    if (!seen.insert(n).second) continue;
+    if (dynamic_cast<torch::autograd::AccumulateGrad*>(n)) check(n);
+    for (const auto& e : n->next_edges())
+      if (e.function) todo.push_back(e.function.get());
   }
 }
 

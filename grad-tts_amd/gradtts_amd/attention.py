@@ -23,8 +23,9 @@ def bucket_attention(q, k, v, table, lengths=None, q_lengths=None, q_start=None,
     and pass no gradient, as do rows that see no key. Query i stands at ``pos_i = q_start[b] + i`` (q_start 0 if None): a
     decoding step over a cache passes ``q_start = lengths - Tq``. causal: keys ``j > pos_i`` are not seen and the buckets
     cover distances ``pos_i - j``; otherwise each direction has half of them (n_buckets even). scale: 1 / sqrt(D) if
-    None. Products and the probabilities entering them are of q's type; sums, statistics and score gradients float32.
-    Works on the current stream; may be captured into a graph. Needs a HIP device."""
+    None, else in [2^-20, 2^20]. Table entries below -2^17 (or -inf) shut their bucket off. Products and the probabilities entering them are of q's type; sums, statistics and score gradients float32.
+    Works on the current stream; may be captured into a graph (with gradients only once no eager autograd graph of the same
+    parameters is alive: refused otherwise). Needs a HIP device."""
     if not q.is_cuda and q.device.type != "meta":
         raise RuntimeError("bucket_attention needs a HIP (MI355X) device; there is no CPU path")
     if scale is None:

@@ -17,7 +17,8 @@ def residual_norm(x, y, post_weight, pre_weight, post_bias=None, pre_bias=None, 
     biases ``[C]``; gate: float32 ``[C]``, or ``[B, C]`` for one of each batch entry, or None (1). All of them are
     differentiable. lengths: integers ``[B]``; rows ``t >= lengths[b]`` are not read, their outputs and gradients are
     zero. Statistics and parameter gradients are float32 sums in a fixed order. Works on the current stream; may be
-    captured into a graph. Needs a HIP device."""
+    captured into a graph (with gradients only once no eager autograd graph of the same parameters is alive: refused
+    otherwise). Needs a HIP device."""
     if not x.is_cuda and x.device.type != "meta":
         raise RuntimeError("residual_norm needs a HIP (MI355X) device; there is no CPU path")
     if kind not in ("layer", "rms"):

@@ -273,6 +273,13 @@ def test_capture_with_gradients_beside_a_living_eager_graph_is_refused():
     with pytest.raises(RuntimeError, match="eager autograd graph"):
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             residual_norm(**args)
+    w = torch.randn(64, 64, device="cuda", requires_grad=True)
+    through = bucket_attention(q.detach() @ w, k, v, table)
+    with pytest.raises(RuntimeError, match="eager autograd graph"):   # the leaf behind an input that is none
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            bucket_attention((q.detach().reshape(-1, 64) * w[0]).view(q.shape), k, v, table)
+    through.sum().backward()
+    del through
     alive.sum().backward()
     (kept[0].sum() + kept[1].sum()).backward()
     assert bool(torch.isfinite(q.grad).all()) and bool(torch.isfinite(args["pre_weight"].grad).all())
