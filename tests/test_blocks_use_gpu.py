@@ -44,6 +44,8 @@ FORMS = [
     (1, 1, 5000, 8, 2, 128, True, 32, 128, None, None, [4999]),
     (3, 2, 1500, 4, 2, 64, True, 32, 128, [1500, 3, 0], None, [1498, 1, 0]),
     (2, 7, 1300, 6, 1, 50, False, 32, 128, [1300, 700], None, [300, 0]),
+    (3, 3, 1500, 4, 2, 64, False, 32, 128, [1500, 900, 1], [2, 0, 3], [100, 0, -5]),
+    (1, 33, 2000, 2, 2, 96, True, 32, 128, [1999], [32], [1960]),
     (2, 1, 600, 32, 1, 64, True, 128, 1024, [600, 40], None, [599, 39]),
     (1, 3, 90, 80, 1, 16, True, 32, 128, None, None, [87]),
     (1, 40, 50, 2, 1, 128, False, 128, 1024, None, None, None),
