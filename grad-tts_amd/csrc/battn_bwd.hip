@@ -573,9 +573,19 @@ template <class T, int DP, int WR> hipError_t bwd_k(BaParams p, const BwdPlan& b
   return launch(ba_dkv_kernel<T, DP, WR, 4 / WR>, grid, 256, SH::BYTES + SH::NBUF * 2 * SH::KT * 4 + host_ext_bytes(p), p, s);
 }
 template <class T, int DP> hipError_t bwd(const BaParams& p, const BwdPlan& b, hipStream_t s) {
-  hipError_t e = b.rows_q == 128 ? bwd_q<T, DP, 4>(p, b, s) : b.rows_q == 64 ? bwd_q<T, DP, 2>(p, b, s) : bwd_q<T, DP, 1>(p, b, s);
-  if (e == hipSuccess)
-    e = b.rows_k == 128 ? bwd_k<T, DP, 4>(p, b, s) : b.rows_k == 64 ? bwd_k<T, DP, 2>(p, b, s) : bwd_k<T, DP, 1>(p, b, s);
+  constexpr bool few = sizeof(T) == 2 || DP <= 64, many = sizeof(T) == 4 || DP < 128;   // as plan_bwd gives them
+  hipError_t e = hipErrorInvalidValue;
+  if (b.rows_q == 64) e = bwd_q<T, DP, 2>(p, b, s);
+  if constexpr (many)
+    if (b.rows_q == 128) e = bwd_q<T, DP, 4>(p, b, s);
+  if constexpr (few)
+    if (b.rows_q == 32) e = bwd_q<T, DP, 1>(p, b, s);
+  if (e != hipSuccess) return e;
+  e = hipErrorInvalidValue;
+  if (b.rows_k == 128) e = bwd_k<T, DP, 4>(p, b, s);
+  if (b.rows_k == 64) e = bwd_k<T, DP, 2>(p, b, s);
+  if constexpr (few)
+    if (b.rows_k == 32) e = bwd_k<T, DP, 1>(p, b, s);
   if (e != hipSuccess) return e;
   if (p.gsplit > 1) {
     const bool four = p.D % 4 == 0;
