@@ -7,6 +7,7 @@
 #include <cmath>
 #include <cstring>
 #include <map>
+#include <memory>
 #include <string>
 #include <vector>
 
@@ -236,11 +237,11 @@ int gt_text_encoder_create_buckets(int n_vocab, int n_feats, int n_channels, int
                                                 "in LayerNorms, odd kernels <= 5, <= 128 features");
   if (gt_relative_bucket(0, n_buckets, max_distance, 0) < 0)
     return gt_internal_fail(GT_ERR_ARG, "n_buckets must be even in [4, 128], max_distance in (n_buckets / 4, 1024]");
-  gt_text_encoder* e = new gt_text_encoder();
+  auto e = std::make_unique<gt_text_encoder>();
   e->n_vocab = n_vocab; e->n_feats = n_feats; e->C = n_channels; e->Fc = filter_channels; e->Fdp = filter_channels_dp;
   e->H = n_heads; e->L = n_layers; e->K = kernel_size; e->W = 0; e->buckets = n_buckets; e->max_distance = max_distance;
-  build_inventory(e);
-  *out = e;
+  build_inventory(e.get());
+  *out = e.release();
   return GT_OK;
 } catch (...) { return gt_internal_fail(GT_ERR_ARG, "gt_text_encoder_create_buckets: out of memory"); }
 
