@@ -5,7 +5,7 @@
 //
 // Many rows: bound by the matrix cores with the exponentials between their products, one wave's softmax beside another's
 // products: 2 x 16 bf16 heads of 4096 causal rows, 64 channels (69 GFLOP) in 90 to 100 us, 0.7 PFLOP/s where a large
-// library product reaches 1.17; 16 heads of 2048 rows, 128 channels in 60. Few rows: bound by memory, 32 sequences of up
+// library product reaches 1.17 (fp16 122); 16 heads of 2048 rows, 128 channels in 60. Few rows: bound by memory, 32 sequences of up
 // to 8192 keys, 4 x 128 channels (342 MB) in 75 us and 5 for the join, 4.5 TB/s where a copy reaches 4.9. Small calls:
 // by latency, some 4 us from the launch to the first product (lengths, rows and table are dependent loads) and, in fp32,
 // 2.6 us of products for each 32 x 32 block of 96 channels: one row over 190 keys 14 us.
@@ -18,13 +18,18 @@ namespace {
 
 // Reference m and sum l of a row's exponentials 2^(score - m), and its sums over v: `block` folds NB 32-key blocks in.
 // SAFE: m is the running maximum, moved once a row's maximum has grown by 8 (in log2 units), and the sums follow it.
-// Otherwise m is the maximum of the row's first keys and stays: neither maxima nor rescaling for any later block. Terms
-// then grow up to the range of fp32 (fp16: of the type, which m starts 2^6 below), which `overflowed` sees in the sums;
-// the rows are then done again the safe way. Nothing is lost below: what lies far under the first maximum does not count.
+// Otherwise (kFixed) m is the maximum of the row's first keys and stays: neither maxima nor rescaling for any later block.
+// Terms then grow up to the range of fp32, which `overflowed` sees in the sums; the rows are then done again the safe way.
+// Nothing is lost below: fp32 and bf16 hold terms down to 2^-126 of the first maximum.
+// fp16 has no such range. It always takes the running maximum, and m lies kBelow = 7 below it: P of the largest term lies
+// in [2^7, 2^15], so the 2^-25 by which rounding P can be off is 2^-32 of the largest term at most, below any sum's
+// own rounding even where one key outweighs thousands (2 x 16 causal heads of 4096 rows, 64 channels: 122 us; a fixed
+// reference took 112 and lost keys 13 nats below an early one).
 template <class T, int DP> struct Softmax {
   typedef typename El<T>::frag frag;
+  static constexpr bool kFixed = !std::is_same<T, f16>::value;
+  static constexpr float kBelow = kFixed ? 0.f : 7.f;
   static constexpr int DB = DP / 32;
-  static constexpr float kRoom = El<T>::wide || __is_same(T, bf16) ? 0.f : 6.f;
   f32x16 o[DB];
   float m, l;
   GT_DEV void clear() {
@@ -54,8 +59,9 @@ template <class T, int DP> struct Softmax {
   }
   // s: scores / c (without off), -inf where unseen; col(n, tt, d): fragment of v for key group tt of block n
   template <bool SAFE, int NB, class Col> GT_DEV void block(const f32x16 (&s)[NB], const float (&off)[NB], float c, Col col) {
+    static_assert(SAFE || kFixed, "range");
     if constexpr (SAFE) {
-      const float mt = largest<NB>(s, off, c), mn = mt > m + 8.f || m == -kInf ? fmaxf(m, mt) : m;
+      const float mt = largest<NB>(s, off, c) - kBelow, mn = mt > m + 8.f || m == -kInf ? fmaxf(m, mt) : m;
       const float al = __builtin_amdgcn_exp2f(m - (mn == -kInf ? 0.f : mn));
       m = mn;
       l *= al;
@@ -65,7 +71,7 @@ template <class T, int DP> struct Softmax {
 #pragma unroll
         for (int j = 0; j < 16; ++j) o[d][j] *= al;
     } else if (__any(m == -kInf)) {
-      float mt = largest<NB>(s, off, c) + kRoom;
+      float mt = largest<NB>(s, off, c);
       in_branch(mt);
       m = m == -kInf ? mt : m;
     }
@@ -214,8 +220,12 @@ __global__ __launch_bounds__(64 * WR * WS, sizeof(T) == 4 ? 1 : 2) void ba_fwd_k
         if (t + 1 < ntile) step(t + 1, std::integral_constant<int, 1>(), safe);
       }
     };
-    run(std::false_type());
-    if (__syncthreads_or(sm.overflowed())) run(std::true_type());
+    if constexpr (Softmax<T, DP>::kFixed) {
+      run(std::false_type());
+      if (__syncthreads_or(sm.overflowed())) run(std::true_type());
+    } else {
+      run(std::true_type());
+    }
     const float l = both_sum(sm.l);
     const long stat = ((long)b * p.Hq + h) * p.Tq + qi;
     T* ob = (T*)p.out + b * p.os.b + h * p.os.h;
