@@ -19,7 +19,7 @@ namespace {
 // Reference m and sum l of a row's exponentials 2^(score - m), and its sums over v: `block` folds NB 32-key blocks in.
 // SAFE: m is the running maximum, moved once a row's maximum has grown by 8 (in log2 units), and the sums follow it.
 // Otherwise (kFixed) m is the maximum of the row's first keys and stays: neither maxima nor rescaling for any later block.
-// Terms then grow up to the range of fp32, which `overflowed` sees in the sums; the rows are then done again the safe way.
+// Terms then grow up to 2^100, which `overflowed` sees in the sums; the rows are then done again the safe way.
 // Nothing is lost below: fp32 and bf16 hold terms down to 2^-126 of the first maximum.
 // fp16 has no such range. It always takes the running maximum, and m lies kBelow = 7 below it: P of the largest term lies
 // in [2^7, 2^15], so the 2^-25 by which rounding P can be off is 2^-32 of the largest term at most, below any sum's
@@ -38,8 +38,9 @@ template <class T, int DP> struct Softmax {
     m = -kInf;
     l = 0.f;
   }
+  // (l well below the end of the range: the sums of the lane halves and of the streams, and 1 / l, are normal numbers)
   GT_DEV bool overflowed() const {
-    bool bad = !(l < kInf);
+    bool bad = !(l < 0x1p100f);
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll

@@ -17,7 +17,7 @@ def _need_gpu():
         pytest.skip("no HIP device")
 
 
-def check_two(name, args, dout, heads, **kw):
+def check_two(name, args, dout, heads, extra=0.0, **kw):
     """args, dout: two heads, each with keys of its own; the call has `heads` of them, the two in turn. Checks the first
     and the last two; returns what was compared."""
     want, bound = blocks.attention(*args, dout, **kw)
@@ -25,7 +25,7 @@ def check_two(name, args, dout, heads, **kw):
     got = attend(*(t.repeat(1, 1, n, 1) for t in args[:3]), args[3].repeat(1, n), dout.repeat(1, 1, n, 1), **kw)
     for part, sl in (("first", slice(0, 2)), ("last", slice(heads - 2, heads))):
         for k in want:
-            close(f"{name} {part} {k}", got[k][:, sl] if k == "dtable" else got[k][:, :, sl], want[k], bound[k])
+            close(f"{name} {part} {k}", got[k][:, sl] if k == "dtable" else got[k][:, :, sl], want[k], bound[k] + extra)
 
 
 # heads, queries: tiles of 128 rows, of 64, packed rows
@@ -45,3 +45,22 @@ def test_first_key_outweighs_thousands(dtype, heads, Tq, gap):
     k[:, 0], v[:, 0] = 0, 0
     k[:, 0, :, 0] = gap * D ** 0.5
     check_two(f"{dtype} gap {gap}", (q, k, v, table), dout, heads, max_distance=3)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("heads, Tq", ROWS)
+@pytest.mark.parametrize("pair", [(100, 104), (100, 132), (36, 67)])
+def test_two_parts_of_a_sum_pass_the_range_together(dtype, heads, Tq, pair):
+    """Two keys some 2^127.7 above the first ones: either one's term is a finite float32, their sum is none. They fall to
+    the two halves of a wave, or to two waves. Values of 1 / 4 and less keep the sums over them finite."""
+    Tk, D = 200, 64
+    q, k, v, table, dout = inputs(32, DT[dtype], 1, Tq, Tk, 2, 2, D, 4)
+    q, k, v, table = 0 * q, 0.1 * k, 0.06 * v, 0 * table
+    q[..., 0], k[..., 0] = 1, 0
+    for j in pair:
+        k[:, j, :, 0] = 708   # 708 / 8 nats = 127.68 powers of two
+    assert 127 < float(k[0, pair[0], 0, 0]) / D ** 0.5 * 1.4426950408889634 < 128 and float(v.abs().max()) < 0.5
+    # the other keys' probabilities, 2^-128, lie below fp32's least normal number and count as zeros, 2^-126 each: times a
+    # factor dP - delta below 2^7 (64 products of at most 5 and 0.5), keys and values below 2^10, and summed over at most
+    # 130 x 200 < 2^15 pairs: below 2^-94 in any gradient
+    check_two(f"{dtype} pair {pair}", (q, k, v, table), dout, heads, 2.0 ** -94, max_distance=3)
