@@ -135,7 +135,7 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 2 || sizeof(T) == 4 ? 1 : 2) voi
       }
     };
     read(0);
-    if (dmax <= -p.dsat || dmin >= p.dsat) {
+    if (one_bias(dmin, dmax, p.dsat, p.causal)) {
       off = dmin < 0 ? blo : bhi;
       s = mma0<T>(a[0], qf[0]);
     } else {
@@ -208,7 +208,7 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 2 || sizeof(T) == 4 ? 1 : 2) voi
       for (int d = 0; d < DB; ++d) kc[d] = TL::col(sk, 32 * j2, d, lane);
 #pragma unroll
       for (int j = 0; j < 16; ++j) ds[j] *= dp[j] - delta;
-      if (dmax <= -p.dsat || dmin >= p.dsat) {
+      if (one_bias(dmin, dmax, p.dsat, p.causal)) {
         float a = 0.f;
 #pragma unroll
         for (int j = 0; j < 16; ++j) a += ds[j];
@@ -388,7 +388,7 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 2 || sizeof(T) == 4 || DP > 64 ?
               }
             };
             read(0);
-            if (dmax <= -p.dsat || dmin >= p.dsat) {
+            if (one_bias(dmin, dmax, p.dsat, p.causal)) {
               off = dmin < 0 ? blo : bhi;
               s = mma0<T>(a[0], kf[0]);
             } else {

@@ -18,6 +18,7 @@
 // WS = 4 spreads few rows over four waves (latency, memory).
 #pragma once
 #include "battn.h"
+#include "battn_index.h"
 
 #include "common.h"
 
@@ -193,17 +194,15 @@ GT_DEV int bucket_of(const BaParams& p, int delta) {   // delta = key position -
     for (int e = 0; e < 8; ++e) b += dist >= p.border[k + e];
   return b + ((!p.causal && delta > 0) ? p.side : 0);
 }
-// LDS table over the offsets -dsat - EXT .. dsat + EXT (causal: .. EXT): a 32 x 32 block with an offset inside
-// (-dsat, dsat) has all of its 63 offsets in it
-constexpr int EXT = 64;
-GT_DEV int ext_len(const BaParams& p) { return p.dsat + 2 * EXT + 1 + (p.causal ? 0 : p.dsat); }
+GT_DEV int ext_len(const BaParams& p) { return ext_entries(p.dsat, p.causal); }
 // Entries below -2^17 shut their bucket off as -inf does (rows that see only such keys are empty), entries above 2^17
 // count as 2^17: exponents stay where one FMA is exact enough
 template <class T> GT_DEV float table_at(const BaParams& p, int bucket, int h) {
   const float x = (float)((const T*)p.table)[(long)bucket * p.Hq + h];
   return x < -131072.f ? -kInf : x > 131072.f ? 131072.f : x;
 }
-// bias / scale of the heads h0 .. h0 + nh - 1 (the last head again past h_last), ext_len entries each
+// LDS tables of bias / scale by offset (battn_index.h) of the heads h0 .. h0 + nh - 1 (the last head again past h_last),
+// ext_len entries each
 template <class T> GT_DEV void build_ext(const BaParams& p, int h0, int nh, int h_last, float* ext, int tid, int nthreads) {
   const int n = ext_len(p);
   for (int i = tid; i < n; i += nthreads) {
@@ -371,7 +370,7 @@ template <class T> GT_DEV void store4_row(T* row, int d, const float* x, int D, 
 }
 
 // ---------------------------------------------------------------- launches
-inline int host_ext_bytes(const BaParams& p) { return (p.dsat + 2 * EXT + 1 + (p.causal ? 0 : p.dsat)) * 4; }
+inline int host_ext_bytes(const BaParams& p) { return ext_entries(p.dsat, p.causal) * 4; }
 // launches over 64 KB of LDS need the kernel's limit raised
 template <class K> hipError_t launch(K kernel, long grid, int threads, int smem, const BaParams& p, hipStream_t s) {
   if (grid > 0x7fffffffL) return hipErrorInvalidValue;

@@ -114,7 +114,7 @@ template <class T, int KS>
 GT_DEV void score_block(const BaParams& p, const Seen& w, int klen, int kk, int hh, const typename El<T>::frag (&a)[KS],
                         const typename El<T>::frag (&qf)[KS], f32x16& s, float& off) {
   const int dmax = kk + 31 - w.pmin, dmin = kk - w.pmax;   // offsets of the block
-  if (dmax <= -p.dsat || dmin >= p.dsat) {   // (causal and past the row: wholly unseen)
+  if (one_bias(dmin, dmax, p.dsat, p.causal)) {
     off = dmin < 0 ? w.blo : w.bhi;
     s = mma0<T>(a[0], qf[0]);
   } else {

@@ -64,3 +64,12 @@ def test_two_parts_of_a_sum_pass_the_range_together(dtype, heads, Tq, pair):
     # factor dP - delta below 2^7 (64 products of at most 5 and 0.5), keys and values below 2^10, and summed over at most
     # 130 x 200 < 2^15 pairs: below 2^-94 in any gradient
     check_two(f"{dtype} pair {pair}", (q, k, v, table), dout, heads, 2.0 ** -94, max_distance=3)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("heads", [512, 64, 2])
+@pytest.mark.parametrize("start", [1, 2, 31, 33, 63])
+def test_causal_chunk_that_starts_between_tiles(dtype, heads, start):
+    """The next 140 tokens of a sequence, `start` of which are in the cache already."""
+    *args, dout = inputs(33, DT[dtype], 1, 140, 140 + start, 2, 2, 40, 32)
+    check_two(f"{dtype} start {start}", args, dout, heads, causal=True, q_start=[start])
