@@ -501,6 +501,42 @@ std::tuple<at::Tensor, at::Tensor> bucket_attention_autograd(const at::Tensor& q
   return {r[0], r[1]};
 }
 
+// The gradients carry a node of their own where grad mode is on (create_graph): it refuses to be differentiated, where
+// operators without one would pass zeros on.
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> bucket_attention_backward_below(
+    const at::Tensor& dout, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& table,
+    const OptTensor& lengths, const OptTensor& q_lengths, const OptTensor& q_start, const at::Tensor& out,
+    const at::Tensor& lse, bool causal, int64_t max_distance, double scale) {
+  static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("gradtts::bucket_attention_backward", "")
+                       .typed<decltype(bucket_attention_backward_hip)>();
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(dout, q, k, v, table, lengths, q_lengths, q_start, out, lse, causal, max_distance, scale);
+}
+struct BucketAttentionBackwardFn : torch::autograd::Function<BucketAttentionBackwardFn> {
+  static variable_list forward(AutogradContext*, const at::Tensor& dout, const at::Tensor& q, const at::Tensor& k,
+                               const at::Tensor& v, const at::Tensor& table, const OptTensor& lengths,
+                               const OptTensor& q_lengths, const OptTensor& q_start, const at::Tensor& out,
+                               const at::Tensor& lse, bool causal, int64_t max_distance, double scale) {
+    auto [dq, dk, dv, dt] = bucket_attention_backward_below(dout, q, k, v, table, lengths, q_lengths, q_start, out, lse,
+                                                            causal, max_distance, scale);
+    return {dq, dk, dv, dt};
+  }
+  static variable_list backward(AutogradContext*, variable_list) {
+    TORCH_CHECK_NOT_IMPLEMENTED(false, "gradtts: bucket_attention has no second derivatives");
+  }
+};
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> bucket_attention_backward_autograd(
+    const at::Tensor& dout, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& table,
+    const OptTensor& lengths, const OptTensor& q_lengths, const OptTensor& q_start, const at::Tensor& out,
+    const at::Tensor& lse, bool causal, int64_t max_distance, double scale) {
+  if (!at::GradMode::is_enabled())
+    return bucket_attention_backward_below(dout, q, k, v, table, lengths, q_lengths, q_start, out, lse, causal,
+                                           max_distance, scale);
+  const auto r = BucketAttentionBackwardFn::apply(dout, q, k, v, table, lengths, q_lengths, q_start, out, lse, causal,
+                                                  max_distance, scale);
+  return {r[0], r[1], r[2], r[3]};
+}
+
 struct ResidualNormFn : torch::autograd::Function<ResidualNormFn> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& y, const OptTensor& gate,
                                const at::Tensor& w1, const OptTensor& b1, const at::Tensor& w2, const OptTensor& b2,
@@ -527,6 +563,40 @@ struct ResidualNormFn : torch::autograd::Function<ResidualNormFn> {
     return {dx, dy, of(s[2], dg), dw1, of(s[4], db1), dw2, of(s[6], db2), Variable(), Variable(), Variable(), Variable()};
   }
 };
+using NormGrads = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
+NormGrads residual_norm_backward_below(const at::Tensor& dout, const at::Tensor& dh, const at::Tensor& x,
+                                       const at::Tensor& y, const OptTensor& gate, const at::Tensor& w1,
+                                       const OptTensor& b1, const at::Tensor& w2, const OptTensor& b2,
+                                       const OptTensor& lengths, const at::Tensor& stats, double scale, double eps,
+                                       bool rms) {
+  static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("gradtts::residual_norm_backward", "")
+                       .typed<decltype(residual_norm_backward_hip)>();
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(dout, dh, x, y, gate, w1, b1, w2, b2, lengths, stats, scale, eps, rms);
+}
+struct ResidualNormBackwardFn : torch::autograd::Function<ResidualNormBackwardFn> {
+  static variable_list forward(AutogradContext*, const at::Tensor& dout, const at::Tensor& dh, const at::Tensor& x,
+                               const at::Tensor& y, const OptTensor& gate, const at::Tensor& w1, const OptTensor& b1,
+                               const at::Tensor& w2, const OptTensor& b2, const OptTensor& lengths,
+                               const at::Tensor& stats, double scale, double eps, bool rms) {
+    auto [dx, dy, dg, dw1, db1, dw2, db2] =
+        residual_norm_backward_below(dout, dh, x, y, gate, w1, b1, w2, b2, lengths, stats, scale, eps, rms);
+    return {dx, dy, dg, dw1, db1, dw2, db2};
+  }
+  static variable_list backward(AutogradContext*, variable_list) {
+    TORCH_CHECK_NOT_IMPLEMENTED(false, "gradtts: residual_norm has no second derivatives");
+  }
+};
+NormGrads residual_norm_backward_autograd(const at::Tensor& dout, const at::Tensor& dh, const at::Tensor& x,
+                                          const at::Tensor& y, const OptTensor& gate, const at::Tensor& w1,
+                                          const OptTensor& b1, const at::Tensor& w2, const OptTensor& b2,
+                                          const OptTensor& lengths, const at::Tensor& stats, double scale, double eps,
+                                          bool rms) {
+  if (!at::GradMode::is_enabled())
+    return residual_norm_backward_below(dout, dh, x, y, gate, w1, b1, w2, b2, lengths, stats, scale, eps, rms);
+  const auto r = ResidualNormBackwardFn::apply(dout, dh, x, y, gate, w1, b1, w2, b2, lengths, stats, scale, eps, rms);
+  return {r[0], r[1], r[2], r[3], r[4], r[5], r[6]};
+}
 std::tuple<at::Tensor, at::Tensor, at::Tensor> residual_norm_autograd(
     const at::Tensor& x, const at::Tensor& y, const OptTensor& gate, const at::Tensor& w1, const OptTensor& b1,
     const at::Tensor& w2, const OptTensor& b2, const OptTensor& lengths, double scale, double eps, bool rms) {
@@ -567,7 +637,9 @@ TORCH_LIBRARY_IMPL(gradtts, CUDA, m) {
 
 TORCH_LIBRARY_IMPL(gradtts, Autograd, m) {
   m.impl("bucket_attention", &bucket_attention_autograd);
+  m.impl("bucket_attention_backward", &bucket_attention_backward_autograd);
   m.impl("residual_norm", &residual_norm_autograd);
+  m.impl("residual_norm_backward", &residual_norm_backward_autograd);
 }
 
 TORCH_LIBRARY_IMPL(gradtts, Meta, m) {

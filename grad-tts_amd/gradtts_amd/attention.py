@@ -18,8 +18,8 @@ def bucket_attention(q, k, v, table, lengths=None, q_lengths=None, q_start=None,
     """``softmax(q k^T scale + table[bucket(j - pos_i)]) v`` for every head; returns ``[B, Tq, Hq, D]`` of q's type.
 
     q ``[B, Tq, Hq, D]``, k and v ``[B, Tk, Hkv, D]`` (Hq a multiple of Hkv, D <= 128; any strides, best with contiguous
-    channels), table ``[n_buckets, Hq]``; all float32, bfloat16 or float16 and differentiable. lengths, q_lengths,
-    q_start: integers ``[B]``. Keys ``j >= lengths[b]`` are neither seen nor read; rows ``i >= q_lengths[b]`` give zeros
+    channels), table ``[n_buckets, Hq]``; all float32, bfloat16 or float16 and differentiable (once: second
+    derivatives raise). lengths, q_lengths, q_start: integers ``[B]``. Keys ``j >= lengths[b]`` are neither seen nor read; rows ``i >= q_lengths[b]`` give zeros
     and pass no gradient, as do rows that see no key. Query i stands at ``pos_i = q_start[b] + i`` (q_start 0 if None): a
     decoding step over a cache passes ``q_start = lengths - Tq``. causal: keys ``j > pos_i`` are not seen and the buckets
     cover distances ``pos_i - j``; otherwise each direction has half of them (n_buckets even). scale: 1 / sqrt(D) if

@@ -1,9 +1,14 @@
-"""Bucket attention without a GPU: offsets that the kernels look up against the extent of their bias table."""
+"""Transformer-block operators without a GPU: offsets that the attention kernels look up against the extent of their bias
+table, second derivatives."""
 import ctypes
 import os
 import subprocess
 
 import pytest
+import torch
+
+from gradtts_amd.attention import bucket_attention
+from gradtts_amd.norm import residual_norm
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "grad-tts_amd", "csrc")
 
@@ -72,3 +77,19 @@ def test_blocks_ahead_of_every_query_would_leave_the_causal_table(outside):
     reads past the table's end."""
     assert outside(113, 1, 64, 2, 32, 32, 1) > 0
     assert outside(113, 0, 64, 2, 32, 32, 1) == 0
+
+
+def test_second_derivatives_are_refused():
+    """Gradients of a graph that is kept are values as any others; what differentiates them raises."""
+    q, k, t = (torch.empty(s, device="meta", requires_grad=True) for s in ((2, 5, 4, 64), (2, 7, 2, 64), (32, 4)))
+    x, w, g = (torch.empty(s, device="meta", requires_grad=True) for s in ((2, 3, 64), (64,), (2, 64)))
+    out = bucket_attention(q, k, k, t)
+    norm = residual_norm(x, x * 2, w, w, gate=g)
+    for outs, leaves, name in ((out, [q, k, t], "bucket_attention"), (norm[0] + norm[1], [x, w, g], "residual_norm")):
+        grads = torch.autograd.grad(outs.sum(), leaves, create_graph=True)
+        assert [d.shape for d in grads] == [p.shape for p in leaves] and all(d.requires_grad for d in grads)
+        for d in grads:
+            with pytest.raises(NotImplementedError, match=f"{name} has no second derivatives"):
+                torch.autograd.grad(d.sum(), leaves, allow_unused=True, retain_graph=True)
+        plain = torch.autograd.grad(outs.sum(), leaves)
+        assert not any(d.requires_grad for d in plain)

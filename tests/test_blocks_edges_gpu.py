@@ -5,8 +5,10 @@ import pytest
 import torch
 
 from conftest import gpu_available
+from gradtts_amd.attention import bucket_attention
+from gradtts_amd.norm import residual_norm
 from oracle import blocks
-from test_blocks_gpu import DT, attend, close, inputs
+from test_blocks_gpu import DT, attend, close, inputs, norm_inputs, norm_step
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +75,22 @@ def test_causal_chunk_that_starts_between_tiles(dtype, heads, start):
     """The next 140 tokens of a sequence, `start` of which are in the cache already."""
     *args, dout = inputs(33, DT[dtype], 1, 140, 140 + start, 2, 2, 40, 32)
     check_two(f"{dtype} start {start}", args, dout, heads, causal=True, q_start=[start])
+
+
+def test_gradients_of_a_kept_graph():
+    """create_graph changes no value; differentiating what it gives raises, eager and compiled code go on working."""
+    q, k, v, table, dout = inputs(34, torch.bfloat16, 2, 40, 40, 4, 2, 64, 32)
+    want = attend(q, k, v, table, dout)
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v, table)]
+    out = bucket_attention(*leaves)
+    got = torch.autograd.grad(out, leaves, dout.cuda(), create_graph=True)
+    assert all(torch.equal(g, want[n]) for n, g in zip(("dq", "dk", "dv", "dtable"), got))
+    with pytest.raises(NotImplementedError, match="second derivatives"):
+        sum(g.float().square().sum() for g in got).backward()
+    args, dout, dh = norm_inputs(35, torch.float32, 2, 30, 96, True, "batch")
+    want = norm_step(args, dout, dh)
+    dev = {n: t.cuda().requires_grad_() for n, t in args.items()}
+    got = torch.autograd.grad(residual_norm(**dev), list(dev.values()), [dout.cuda(), dh.cuda()], create_graph=True)
+    assert all(torch.equal(g, want["d" + n]) for n, g in zip(dev, got))
+    with pytest.raises(NotImplementedError, match="second derivatives"):
+        torch.autograd.grad(got[0].square().sum(), dev["x"])
