@@ -67,7 +67,7 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 2 || sizeof(T) == 4 ? 1 : 2) voi
   float* sat = ext0 + (1 + NW) * elen;                   // [NW][2]; [NW][32] before
   const int nbk = p.B * p.Hkv, bk = blockIdx.x % (unsigned)nbk, rest = blockIdx.x / (unsigned)nbk, b = bk / p.Hkv, hk = bk % p.Hkv;
   const int h = hk * p.G + rest % p.G, rank = rest / p.G;
-  const int qlen = clamp_len(p.qlen, b, p.Tq), klen = clamp_len(p.len, b, p.Tk), pos0 = start_of(p, b);
+  const int qlen = clamp_len(p.qlen, b, p.Tq), pos0 = start_of(p, b), klen = keys_of(p, b, qlen, pos0);
   const T* kb = (const T*)p.k + b * p.ks.b + hk * p.ks.h;
   const T* vb = (const T*)p.v + b * p.vs.b + hk * p.vs.h;
   auto tile = [&](int t, int which) { return smem + ((SH::NBUF == 2 ? t & 1 : 0) * 2 + which) * SH::TILE; };
@@ -307,7 +307,7 @@ __global__ __launch_bounds__(64 * WR * WS, WS > 2 || sizeof(T) == 4 || DP > 64 ?
   const int tid = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wv % WR, ws = wv / WR;
   const int nbk = p.B * p.Hkv, bk = blockIdx.x % (unsigned)nbk, rest = blockIdx.x / (unsigned)nbk, b = bk / p.Hkv, hk = bk % p.Hkv;
   const int gpart = rest % p.gsplit, rank = rest / p.gsplit;
-  const int qlen = clamp_len(p.qlen, b, p.Tq), klen = clamp_len(p.len, b, p.Tk), pos0 = start_of(p, b);
+  const int qlen = clamp_len(p.qlen, b, p.Tq), pos0 = start_of(p, b), klen = keys_of(p, b, qlen, pos0);
 #pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {   // a tile from the start and, paired, its mirror image
     if (pass && (!p.pair || 2 * rank >= p.ntile - 1)) break;

@@ -220,6 +220,12 @@ GT_DEV int start_of(const BaParams& p, int b) {   // far beyond any offset that 
   const int64_t s = p.qstart ? p.qstart[b] : 0;
   return s < -(1 << 29) ? -(1 << 29) : s > (1 << 29) ? (1 << 29) : (int)s;
 }
+// keys of a batch entry that any of its queries sees: none past the last query's position under a causal mask, so what
+// lies behind it in a cache (which zero probabilities would turn into NaN if it were not finite) is not read
+GT_DEV int keys_of(const BaParams& p, int b, int qlen, int pos0) {
+  const int n = clamp_len(p.len, b, p.Tk);
+  return p.causal ? min(n, max(pos0 + qlen, 0)) : n;
+}
 
 // Work item -> batch, heads and tile: batch entry and key / value head go round first, so that the workgroups that read
 // the same keys run on the same XCD (workgroups go round the 8 XCDs in turn). Under a causal mask a workgroup takes a tile

@@ -153,7 +153,7 @@ __global__ __launch_bounds__(64 * WR * WS, sizeof(T) == 4 ? 1 : 2) void ba_fwd_k
   const int h = hk * p.G + rest % p.G, rank = rest / p.G;
   float* ext0 = (float*)(smem + SH::BYTES);
   build_ext<T>(p, h, 1, h, ext0, tid, NT);
-  const int qlen = clamp_len(p.qlen, b, p.Tq), klen = clamp_len(p.len, b, p.Tk), pos0 = start_of(p, b);
+  const int qlen = clamp_len(p.qlen, b, p.Tq), pos0 = start_of(p, b), klen = keys_of(p, b, qlen, pos0);
   const T* kb = (const T*)p.k + b * p.ks.b + hk * p.ks.h;
   const T* vb = (const T*)p.v + b * p.vs.b + hk * p.vs.h;
   auto tile = [&](int t, int which) { return smem + ((SH::NBUF == 2 ? t & 1 : 0) * 2 + which) * SH::TILE; };   // LDS
@@ -286,7 +286,7 @@ __global__ __launch_bounds__(64 * WSP, sizeof(T) == 2 || DP <= 96 ? 2 : 1) void 
   const int split = blockIdx.x / units;
   const int bk = blk % (unsigned)nbk, rest = blk / (unsigned)nbk, b = bk / p.Hkv, hk = bk % p.Hkv;
   const int g0 = rest % ngb * p.gp, i0 = (p.ntile - 1 - rest / ngb) * p.qpb, gp = p.gp;
-  const int qlen = clamp_len(p.qlen, b, p.Tq), klen = clamp_len(p.len, b, p.Tk), pos0 = start_of(p, b);
+  const int qlen = clamp_len(p.qlen, b, p.Tq), pos0 = start_of(p, b), klen = keys_of(p, b, qlen, pos0);
   float* ext0 = (float*)(smem + SP::BYTES);
   build_ext<T>(p, hk * p.G + g0, gp, hk * p.G + p.G - 1, ext0, tid, NT);
   const int gg = (unsigned)r % (unsigned)gp, qi = i0 + min((int)((unsigned)r / (unsigned)gp), p.qpb - 1), h = hk * p.G + min(g0 + gg, p.G - 1);

@@ -94,3 +94,25 @@ def test_gradients_of_a_kept_graph():
     assert all(torch.equal(g, want["d" + n]) for n, g in zip(dev, got))
     with pytest.raises(NotImplementedError, match="second derivatives"):
         torch.autograd.grad(got[0].square().sum(), dev["x"])
+
+
+# B, Tq, Tk, heads, keys the last query sees: packed rows, with key ranges of their own, tiles of 64 and 128 rows; the
+# last query inside a 32-key block
+CACHES = [(2, 1, 200, 2, 70), (1, 1, 3000, 2, 1500), (2, 3, 1400, 4, 1301), (1, 130, 400, 64, 201), (1, 130, 300, 512, 139),
+          (1, 130, 300, 512, 21)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("case", CACHES, ids=str)
+def test_a_cache_is_not_read_behind_the_last_query(dtype, case):
+    """A causal step over a cache whose unwritten part holds NaN and infinities, without lengths: bit for bit what the
+    written part alone gives; the unwritten keys' gradients are zeros."""
+    B, Tq, Tk, H, n = case
+    q, k, v, table, dout = inputs(36, DT[dtype], B, Tq, Tk, H, H, 40, 32)
+    start = torch.tensor([n - Tq] * B)   # below zero: the first rows see no key
+    want = attend(q, k, v, table, dout, causal=True, q_start=start.tolist(), lengths=[n] * B)
+    k[:, n:], v[:, n::2], v[:, n + 1::2] = float("nan"), float("inf"), float("nan")
+    got = attend(q, k, v, table, dout, causal=True, q_start=start.tolist())
+    for name in want:
+        assert torch.equal(got[name], want[name]), name
+    assert not bool(got["dk"][:, n:].any()) and not bool(got["dv"][:, n:].any())
