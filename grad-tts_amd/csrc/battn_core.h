@@ -344,7 +344,7 @@ template <class T, int DP, int WR, int WS> struct Shape {
 
 // Sum over the WS waves of a row block, through LDS ([row block][wave][channel][33], the tiles are done with): afterwards
 // each thread of the row block's waves holds four channels of a row at a time, handed to `out(row, d, x[4])`. `mul`:
-// this wave's factor for its row (lane & 31).
+// this wave's factor for its row (lane & 31); 0: none of the wave's sums count, finite or not (a row that saw no key).
 template <int DP, int WS, class F>
 GT_DEV void join(char* smem, const f32x16 (&acc)[DP / 32], float mul, int wr, int ws, int lane, F out) {
   float* s = (float*)smem + wr * (WS * DP * 33);
@@ -353,7 +353,7 @@ GT_DEV void join(char* smem, const f32x16 (&acc)[DP / 32], float mul, int wr, in
 #pragma unroll
   for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
-    for (int j = 0; j < 16; ++j) s[(ws * DP + 32 * db + acc_row(j, hh)) * 33 + r] = acc[db][j] * mul;
+    for (int j = 0; j < 16; ++j) s[(ws * DP + 32 * db + acc_row(j, hh)) * 33 + r] = mul == 0.f ? 0.f : acc[db][j] * mul;
   __syncthreads();
   for (int i = ws * 64 + lane; i < 32 * DP / 4; i += 64 * WS) {
     const int row = i / (DP / 4), d = i % (DP / 4) * 4;

@@ -116,3 +116,13 @@ def test_a_cache_is_not_read_behind_the_last_query(dtype, case):
     for name in want:
         assert torch.equal(got[name], want[name]), name
     assert not bool(got["dk"][:, n:].any()) and not bool(got["dv"][:, n:].any())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("heads, Tq, Tk", [(512, 130, 130), (64, 130, 130), (2, 40, 40), (1, 5, 1500)])
+def test_rows_before_the_first_key_beside_infinite_values(dtype, heads, Tq, Tk):
+    """Rows that see no key are zeros whatever the keys' values are."""
+    q, k, v, table, _ = inputs(37, DT[dtype], 1, Tq, Tk, heads, heads, 40, 32)
+    v[:, 0] = float("inf")
+    out = attend(q, k, v, table, causal=True, q_start=[-3])["out"]
+    assert not bool(out[:, :3].any()) and bool((out[:, 3] == float("inf")).all())
