@@ -466,6 +466,9 @@ int gt_path_gather(const float* attn, const float* mu_x, int64_t B, int64_t Tx, 
 // ================================================================ training pass (GradTTS.compute_loss's encoder)
 namespace {
 
+// longest sequence of the training pass: the window form's attention keeps a row of scores in LDS, the bucket form none
+int64_t train_tmax(const gt_text_encoder* e) { return e->buckets ? int64_t(1) << 28 : TT_TMAX; }
+
 // tape + backward scratch (floats unless noted), 256-byte aligned pieces
 struct TrWs {
   size_t tokens, mask, x0, pre_c[3], pre_h[3], x1, d1c, d1d, d2c, d2d;
@@ -539,7 +542,7 @@ float* tape_ptr(const TrWs& w, char* base, size_t o, size_t ws_usable, bool& bad
 extern "C" {
 
 size_t gt_text_encoder_train_workspace_bytes(gt_text_encoder* e, int64_t B, int64_t T) {
-  if (!e || B <= 0 || T <= 0 || T > TT_TMAX) return 0;
+  if (!e || B <= 0 || T <= 0 || T > train_tmax(e)) return 0;
   return tr_layout(e, B, T).total;
 }
 
@@ -550,7 +553,7 @@ int gt_text_encoder_forward_train(gt_text_encoder* e, const int64_t* tokens, con
                                   float* logw, float* x_mask, void* workspace, size_t workspace_bytes, void* stream) {
   if (!e || !tokens || !x_lengths || !mu_x || !logw || !x_mask || !workspace) return gt_internal_fail(GT_ERR_ARG, "null argument");
   if (B <= 0 || T <= 0) return gt_internal_fail(GT_ERR_ARG, "bad B / T");
-  if (T > TT_TMAX) return gt_internal_fail(GT_ERR_UNSUPPORTED, "training attention supports Tx <= 4096");
+  if (T > train_tmax(e)) return gt_internal_fail(GT_ERR_UNSUPPORTED, "training attention supports Tx <= 4096");
   if (!(p_dropout >= 0.f && p_dropout < 1.f && p_dropout_prenet >= 0.f && p_dropout_prenet < 1.f))
     return gt_internal_fail(GT_ERR_ARG, "dropout probabilities must lie in [0, 1)");
   const TrWs w = tr_layout(e, B, T);
@@ -695,7 +698,7 @@ int gt_text_encoder_backward(gt_text_encoder* e, const float* dmu_x, const float
                              float p_dropout, float p_dropout_prenet, uint64_t seed, float* grads, void* workspace,
                              size_t workspace_bytes, void* stream) {
   if (!e || !grads || !workspace) return gt_internal_fail(GT_ERR_ARG, "null argument");
-  if (B <= 0 || T <= 0 || T > TT_TMAX) return gt_internal_fail(GT_ERR_ARG, "bad B / T");
+  if (B <= 0 || T <= 0 || T > train_tmax(e)) return gt_internal_fail(GT_ERR_ARG, "bad B / T");
   const TrWs w = tr_layout(e, B, T);
   if (workspace_bytes < w.total) return gt_internal_fail(GT_ERR_WORKSPACE, "workspace too small");
   hipStream_t s = (hipStream_t)stream;

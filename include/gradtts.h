@@ -246,7 +246,8 @@ int gt_path_gather(const float* attn, const float* mu_x, int64_t B, int64_t Tx, 
  * text_encoder.py:321-335) and its backward. gt_text_encoder_forward_train = gt_text_encoder_forward plus the
  * training dropouts (p_dropout: attention probabilities, attention / FFN outputs, FFN hidden, duration predictor;
  * p_dropout_prenet: ConvReluNorm's 0.5; 0 = eval semantics) drawn from `seed` by the library's counter-based
- * generator, and a tape of the activations in `workspace` (gt_text_encoder_train_workspace_bytes). Tx <= 4096.
+ * generator, and a tape of the activations in `workspace` (gt_text_encoder_train_workspace_bytes). Tx <= 4096
+ * (bucket form: any).
  * gt_text_encoder_backward: given dmu_x [B,n_feats,Tx] and dlogw [B,1,Tx] (either may be NULL = zero), writes the
  * gradient of every encoder parameter into grads (gt_text_encoder_grad_numel floats, state_dict inventory order,
  * reference layouts); the duration predictor sees a detached input (text_encoder.py:332), so dlogw reaches only its

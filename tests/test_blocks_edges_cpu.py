@@ -7,6 +7,7 @@ import subprocess
 import pytest
 import torch
 
+from gradtts_amd import _lib
 from gradtts_amd.attention import bucket_attention
 from gradtts_amd.norm import residual_norm
 
@@ -93,3 +94,18 @@ def test_second_derivatives_are_refused():
                 torch.autograd.grad(d.sum(), leaves, allow_unused=True, retain_graph=True)
         plain = torch.autograd.grad(outs.sum(), leaves)
         assert not any(d.requires_grad for d in plain)
+
+
+def test_bucket_encoder_trains_on_long_texts():
+    """The window form's training pass ends at 4096 tokens, where its row of scores fills its memory; the bucket form's
+    keeps no such row: it takes longer ones, in memory that grows with their length alone."""
+    L = _lib.lib()
+    sizes = (61, 80, 192, 768, 256, 2, 2, 3)
+    for create, last, ends in ((L.gt_text_encoder_create, (4,), True), (L.gt_text_encoder_create_buckets, (32, 128), False)):
+        h = ctypes.c_void_p()
+        assert create(*sizes, *last, ctypes.byref(h)) == _lib.GT_OK
+        try:
+            at, past, far = (L.gt_text_encoder_train_workspace_bytes(h, 1, t) for t in (4096, 4097, 16384))
+            assert at > 0 and (past == far == 0 if ends else at < past and far < 4.1 * at)
+        finally:
+            L.gt_text_encoder_destroy(h)
