@@ -126,3 +126,20 @@ def test_rows_before_the_first_key_beside_infinite_values(dtype, heads, Tq, Tk):
     v[:, 0] = float("inf")
     out = attend(q, k, v, table, causal=True, q_start=[-3])["out"]
     assert not bool(out[:, :3].any()) and bool((out[:, 3] == float("inf")).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("B, T", [(8, 190), (40, 140), (4, 60)])
+def test_an_entry_alone_and_in_a_batch(dtype, B, T):
+    """The forms are chosen by the number of rows, so an entry's digits may depend on its batch: both stay within the
+    same bounds, and each call repeats bit for bit."""
+    q, k, v, table, dout = inputs(38, DT[dtype], B, T, T, 16, 8, 40, 32)
+    last = [t[-1:].contiguous() for t in (q, k, v)]
+    want, bound = blocks.attention(*last, table, dout[-1:], causal=True)
+    del want["dtable"]   # a sum over the batch
+    batch, again = (attend(q, k, v, table, dout, causal=True) for _ in range(2))
+    alone = attend(*last, table, dout[-1:], causal=True)
+    assert all(torch.equal(batch[n], again[n]) for n in batch)
+    for n in want:
+        close(f"{dtype} in a batch {n}", batch[n][-1:], want[n], bound[n])
+        close(f"{dtype} alone {n}", alone[n], want[n], bound[n])
