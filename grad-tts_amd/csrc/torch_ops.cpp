@@ -467,40 +467,6 @@ using torch::autograd::variable_list;
 OptTensor opt(const at::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 at::Tensor undef(const OptTensor& t) { return t.has_value() ? *t : at::Tensor(); }
 
-struct BucketAttentionFn : torch::autograd::Function<BucketAttentionFn> {
-  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                               const at::Tensor& table, const OptTensor& lengths, const OptTensor& q_lengths,
-                               const OptTensor& q_start, bool causal, int64_t max_distance, double scale) {
-    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("gradtts::bucket_attention", "")
-                         .typed<decltype(bucket_attention_hip)>();
-    at::AutoDispatchBelowADInplaceOrView below;
-    auto [out, lse] = op.call(q, k, v, table, lengths, q_lengths, q_start, causal, max_distance, scale);
-    ctx->save_for_backward({q, k, v, table, undef(lengths), undef(q_lengths), undef(q_start), out, lse});
-    ctx->saved_data["causal"] = causal;
-    ctx->saved_data["max_distance"] = max_distance;
-    ctx->saved_data["scale"] = scale;
-    ctx->mark_non_differentiable({lse});
-    return {out, lse};
-  }
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("gradtts::bucket_attention_backward", "")
-                         .typed<decltype(bucket_attention_backward_hip)>();
-    const auto s = ctx->get_saved_variables();
-    auto [dq, dk, dv, dt] = op.call(grads[0], s[0], s[1], s[2], s[3], opt(s[4]), opt(s[5]), opt(s[6]), s[7], s[8],
-                                    ctx->saved_data["causal"].toBool(), ctx->saved_data["max_distance"].toInt(),
-                                    ctx->saved_data["scale"].toDouble());
-    return {dq, dk, dv, dt, Variable(), Variable(), Variable(), Variable(), Variable(), Variable()};
-  }
-};
-std::tuple<at::Tensor, at::Tensor> bucket_attention_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                                                             const at::Tensor& table, const OptTensor& lengths,
-                                                             const OptTensor& q_lengths, const OptTensor& q_start,
-                                                             bool causal, int64_t max_distance, double scale) {
-  check_capture({&q, &k, &v, &table});
-  const auto r = BucketAttentionFn::apply(q, k, v, table, lengths, q_lengths, q_start, causal, max_distance, scale);
-  return {r[0], r[1]};
-}
-
 // The gradients carry a node of their own where grad mode is on (create_graph): it refuses to be differentiated, where
 // operators without one would pass zeros on.
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> bucket_attention_backward_below(
@@ -537,32 +503,38 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> bucket_attention_back
   return {r[0], r[1], r[2], r[3]};
 }
 
-struct ResidualNormFn : torch::autograd::Function<ResidualNormFn> {
-  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& y, const OptTensor& gate,
-                               const at::Tensor& w1, const OptTensor& b1, const at::Tensor& w2, const OptTensor& b2,
-                               const OptTensor& lengths, double scale, double eps, bool rms) {
-    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("gradtts::residual_norm", "")
-                         .typed<decltype(residual_norm_hip)>();
+struct BucketAttentionFn : torch::autograd::Function<BucketAttentionFn> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                               const at::Tensor& table, const OptTensor& lengths, const OptTensor& q_lengths,
+                               const OptTensor& q_start, bool causal, int64_t max_distance, double scale) {
+    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("gradtts::bucket_attention", "")
+                         .typed<decltype(bucket_attention_hip)>();
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [out, h, stats] = op.call(x, y, gate, w1, b1, w2, b2, lengths, scale, eps, rms);
-    ctx->save_for_backward({x, y, undef(gate), w1, undef(b1), w2, undef(b2), undef(lengths), stats});
+    auto [out, lse] = op.call(q, k, v, table, lengths, q_lengths, q_start, causal, max_distance, scale);
+    ctx->save_for_backward({q, k, v, table, undef(lengths), undef(q_lengths), undef(q_start), out, lse});
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["max_distance"] = max_distance;
     ctx->saved_data["scale"] = scale;
-    ctx->saved_data["eps"] = eps;
-    ctx->saved_data["rms"] = rms;
-    ctx->mark_non_differentiable({stats});
-    return {out, h, stats};
+    ctx->mark_non_differentiable({lse});
+    return {out, lse};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("gradtts::residual_norm_backward", "")
-                         .typed<decltype(residual_norm_backward_hip)>();
     const auto s = ctx->get_saved_variables();
-    auto [dx, dy, dg, dw1, db1, dw2, db2] =
-        op.call(grads[0], grads[1], s[0], s[1], opt(s[2]), s[3], opt(s[4]), s[5], opt(s[6]), opt(s[7]), s[8],
-                ctx->saved_data["scale"].toDouble(), ctx->saved_data["eps"].toDouble(), ctx->saved_data["rms"].toBool());
-    auto of = [](const at::Tensor& has, const at::Tensor& g) { return has.defined() ? g : Variable(); };
-    return {dx, dy, of(s[2], dg), dw1, of(s[4], db1), dw2, of(s[6], db2), Variable(), Variable(), Variable(), Variable()};
+    auto [dq, dk, dv, dt] = bucket_attention_backward_autograd(
+        grads[0], s[0], s[1], s[2], s[3], opt(s[4]), opt(s[5]), opt(s[6]), s[7], s[8], ctx->saved_data["causal"].toBool(),
+        ctx->saved_data["max_distance"].toInt(), ctx->saved_data["scale"].toDouble());
+    return {dq, dk, dv, dt, Variable(), Variable(), Variable(), Variable(), Variable(), Variable()};
   }
 };
+std::tuple<at::Tensor, at::Tensor> bucket_attention_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                             const at::Tensor& table, const OptTensor& lengths,
+                                                             const OptTensor& q_lengths, const OptTensor& q_start,
+                                                             bool causal, int64_t max_distance, double scale) {
+  check_capture({&q, &k, &v, &table});
+  const auto r = BucketAttentionFn::apply(q, k, v, table, lengths, q_lengths, q_start, causal, max_distance, scale);
+  return {r[0], r[1]};
+}
+
 using NormGrads = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
 NormGrads residual_norm_backward_below(const at::Tensor& dout, const at::Tensor& dh, const at::Tensor& x,
                                        const at::Tensor& y, const OptTensor& gate, const at::Tensor& w1,
@@ -597,6 +569,31 @@ NormGrads residual_norm_backward_autograd(const at::Tensor& dout, const at::Tens
   const auto r = ResidualNormBackwardFn::apply(dout, dh, x, y, gate, w1, b1, w2, b2, lengths, stats, scale, eps, rms);
   return {r[0], r[1], r[2], r[3], r[4], r[5], r[6]};
 }
+
+struct ResidualNormFn : torch::autograd::Function<ResidualNormFn> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& y, const OptTensor& gate,
+                               const at::Tensor& w1, const OptTensor& b1, const at::Tensor& w2, const OptTensor& b2,
+                               const OptTensor& lengths, double scale, double eps, bool rms) {
+    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("gradtts::residual_norm", "")
+                         .typed<decltype(residual_norm_hip)>();
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [out, h, stats] = op.call(x, y, gate, w1, b1, w2, b2, lengths, scale, eps, rms);
+    ctx->save_for_backward({x, y, undef(gate), w1, undef(b1), w2, undef(b2), undef(lengths), stats});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["rms"] = rms;
+    ctx->mark_non_differentiable({stats});
+    return {out, h, stats};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    auto [dx, dy, dg, dw1, db1, dw2, db2] = residual_norm_backward_autograd(
+        grads[0], grads[1], s[0], s[1], opt(s[2]), s[3], opt(s[4]), s[5], opt(s[6]), opt(s[7]), s[8],
+        ctx->saved_data["scale"].toDouble(), ctx->saved_data["eps"].toDouble(), ctx->saved_data["rms"].toBool());
+    auto of = [](const at::Tensor& has, const at::Tensor& g) { return has.defined() ? g : Variable(); };
+    return {dx, dy, of(s[2], dg), dw1, of(s[4], db1), dw2, of(s[6], db2), Variable(), Variable(), Variable(), Variable()};
+  }
+};
 std::tuple<at::Tensor, at::Tensor, at::Tensor> residual_norm_autograd(
     const at::Tensor& x, const at::Tensor& y, const OptTensor& gate, const at::Tensor& w1, const OptTensor& b1,
     const at::Tensor& w2, const OptTensor& b2, const OptTensor& lengths, double scale, double eps, bool rms) {
