@@ -7,8 +7,10 @@
 //
 // Bound by the waves' own latency: at 128 channels the stationary rows, their sums and a block's fragments fill the
 // registers of one wave a SIMD (dK dV) or two (dQ), so products wait for LDS reads and exponentials more than they
-// overlap with them. 2 x 16 bf16 heads (4 key / value heads) of 2048 causal rows, 128 channels: dQ 96 us (0.54 PFLOP/s),
-// dK dV 117 (0.59), sums of head groups 14 (4.8 TB/s), table 5; 3 x 6 fp16 heads of a ragged 777, 80 channels: 40, 36, -, 4.
+// overlap with them. 2 x 16 bf16 heads (4 key / value heads) of 2048 causal rows, 128 channels: dQ 93 us (0.55 PFLOP/s),
+// dK dV 105 (0.65), sums of head groups 14 (4.8 TB/s), table 5; 3 x 6 fp16 heads of 777 rows, 80 channels: 40, 35, -, 4.
+// Registers spill in some forms: 7 in the 16-bit dQ of 128 channels, 9 to 11 in the 16-bit dK dV of 64 channels and 128
+// rows, 67 to 86 in the fp32 dK dV of 128 channels (2 x 16 heads, 4 key / value heads, 1024 causal rows: 296 us).
 #include <type_traits>
 
 #include "battn_core.h"

@@ -5,9 +5,11 @@
 //
 // Many rows: bound by the matrix cores with the exponentials between their products, one wave's softmax beside another's
 // products: 2 x 16 bf16 heads of 4096 causal rows, 64 channels (69 GFLOP) in 90 to 100 us, 0.7 PFLOP/s where a large
-// library product reaches 1.17 (fp16 122); 16 heads of 2048 rows, 128 channels in 60. Few rows: bound by memory, 32 sequences of up
-// to 8192 keys, 4 x 128 channels (342 MB) in 75 us and 5 for the join, 4.5 TB/s where a copy reaches 4.9. Small calls:
-// by latency, some 4 us from the launch to the first product (lengths, rows and table are dependent loads) and, in fp32,
+// library product reaches 1.17 (fp16 122); 16 heads of 2048 rows, 128 channels in 60 (there 2 to 44 registers spill). Rows
+// off the 16-byte grid are read element by element: 2 x 16 causal bf16 heads of 2048 rows take 76 us with 104 channels,
+// 376 with 100. Few rows: bound by memory, 32 sequences of up to 8192 keys, 4 x 128 channels (342 MB) in 75 us and 5 for
+// the join, 4.5 TB/s where a copy reaches 4.9; in fp32, without copies in flight, up to 4096 keys (342 MB) in 130. Small
+// calls: by latency, some 4 us from the launch to the first product (lengths, rows and table are dependent loads) and, in fp32,
 // 2.6 us of products for each 32 x 32 block of 96 channels: one row over 190 keys 14 us.
 #include <type_traits>
 
@@ -19,7 +21,8 @@ namespace {
 // Reference m and sum l of a row's exponentials 2^(score - m), and its sums over v: `block` folds NB 32-key blocks in.
 // SAFE: m is the running maximum, moved once a row's maximum has grown by 8 (in log2 units), and the sums follow it.
 // Otherwise (kFixed) m is the maximum of the row's first keys and stays: neither maxima nor rescaling for any later block.
-// Terms then grow up to 2^100, which `overflowed` sees in the sums; the rows are then done again the safe way.
+// Terms then grow up to 2^100 (69 nats), which `overflowed` sees in the sums; the workgroup's rows are then all done again
+// the safe way: such a call takes about twice as long.
 // Nothing is lost below: fp32 and bf16 hold terms down to 2^-126 of the first maximum.
 // fp16 has no such range. It always takes the running maximum, and m lies kBelow = 7 below it: P of the largest term lies
 // in [2^7, 2^15], so the 2^-25 by which rounding P can be off is 2^-32 of the largest term at most, below any sum's

@@ -18,14 +18,20 @@ def bucket_attention(q, k, v, table, lengths=None, q_lengths=None, q_start=None,
     """``softmax(q k^T scale + table[bucket(j - pos_i)]) v`` for every head; returns ``[B, Tq, Hq, D]`` of q's type.
 
     q ``[B, Tq, Hq, D]``, k and v ``[B, Tk, Hkv, D]`` (Hq a multiple of Hkv, D <= 128; any strides, best with contiguous
-    channels), table ``[n_buckets, Hq]``; all float32, bfloat16 or float16 and differentiable (once: second
-    derivatives raise). lengths, q_lengths, q_start: integers ``[B]``. Keys ``j >= lengths[b]`` are neither seen nor read; rows ``i >= q_lengths[b]`` give zeros
-    and pass no gradient, as do rows that see no key. Query i stands at ``pos_i = q_start[b] + i`` (q_start 0 if None): a
-    decoding step over a cache passes ``q_start = lengths - Tq``. causal: keys ``j > pos_i`` are not seen and the buckets
-    cover distances ``pos_i - j``; otherwise each direction has half of them (n_buckets even). scale: 1 / sqrt(D) if
-    None, else in [2^-20, 2^20]. Table entries below -2^17 (or -inf) shut their bucket off. Products and the probabilities entering them are of q's type; sums, statistics and score gradients float32.
-    Works on the current stream; may be captured into a graph (with gradients only once no eager autograd graph of the same
-    parameters is alive: refused otherwise). Needs a HIP device."""
+    channels and rows on 16 bytes), table ``[n_buckets, Hq]``; all float32, bfloat16 or float16 and differentiable (once:
+    second derivatives raise). lengths, q_lengths, q_start: integers ``[B]``. Keys ``j >= lengths[b]`` are neither seen
+    nor read; rows ``i >= q_lengths[b]`` give zeros and pass no gradient, as do rows that see no key. Query i stands at
+    ``pos_i = q_start[b] + i`` (q_start 0 if None): a decoding step over a cache passes ``q_start = lengths - Tq``.
+    causal: keys ``j > pos_i`` are not seen (nor, past the last query, read) and the buckets cover distances
+    ``pos_i - j``; otherwise each direction has half of them (n_buckets even). scale: 1 / sqrt(D) if None, else in
+    [2^-20, 2^20]. Table entries below -2^17 (or -inf) shut their bucket off.
+
+    Products take q's type: the probabilities and score gradients that enter them are rounded to it; sums and statistics
+    are float32. An infinity or NaN in v may also reach rows of its head and batch entry that see other keys only (zero
+    times infinity). Calls of equal shapes repeat bit for bit; an entry's last digits may depend on the batch around it,
+    whose size chooses the kernel. Scores that rise by some 69 and more past those of a row's first keys make the forward
+    take about twice as long (float16: never). Works on the current stream; may be captured into a graph (with gradients
+    only once no eager autograd graph of the same parameters is alive: refused otherwise). Needs a HIP device."""
     if not q.is_cuda and q.device.type != "meta":
         raise RuntimeError("bucket_attention needs a HIP (MI355X) device; there is no CPU path")
     if scale is None:

@@ -12,11 +12,11 @@ def residual_norm(x, y, post_weight, pre_weight, post_bias=None, pre_bias=None, 
                   kind="layer", lengths=None):
     """``out = x + scale * gate * N1(y)``, ``h = N2(out)``; returns ``(out, h)``.
 
-    x (residual stream) and y (block output) ``[B, T, C]``, float32, bfloat16 or float16, C <= 8192. N is a layer norm
+    x (residual stream) and y (block output) ``[B, T, C]``, float32, bfloat16 or float16, B <= 65535, C <= 8192. N is a layer norm
     (``kind="layer"``) or root-mean-square norm (``"rms"``) over the channels with float32 weights ``[C]`` and optional
     biases ``[C]``; gate: float32 ``[C]``, or ``[B, C]`` for one of each batch entry, or None (1). All of them are
-    differentiable (once: second derivatives raise). lengths: integers ``[B]``; rows ``t >= lengths[b]`` are not read, their outputs and gradients are
-    zero. Statistics and parameter gradients are float32 sums in a fixed order. Works on the current stream; may be
+    differentiable (once: second derivatives raise). lengths: integers ``[B]``; rows ``t >= lengths[b]`` are not read,
+    their outputs and gradients are zero. Statistics and parameter gradients are float32 sums in a fixed order. Works on the current stream; may be
     captured into a graph (with gradients only once no eager autograd graph of the same parameters is alive: refused
     otherwise). Needs a HIP device."""
     if not x.is_cuda and x.device.type != "meta":

@@ -137,7 +137,8 @@ class TextEncoder(torch.nn.Module):
     ``n_buckets`` (with ``window_size=None``) builds the bucket form: the layers attend with a learned bias per bucket
     of distances (``gradtts_amd.attention.bucket_attention``) up to ``max_distance`` instead of relative embeddings
     within a window, and their blocks are joined by ``gradtts_amd.norm.residual_norm`` steps. Heads may have any size
-    up to 128. Its training pass keeps no attention probabilities, so ``p_dropout`` does not fall on them.
+    up to 128. Its training pass keeps no attention probabilities, so ``p_dropout`` does not fall on them and texts may
+    have any length (the window form trains on up to 4096 tokens).
 
     With gradients enabled and parameters that require them, or in train mode with p_dropout > 0, ``forward`` is the
     training pass

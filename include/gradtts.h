@@ -344,7 +344,8 @@ typedef struct { int64_t b, t, h; } gt_stride;   /* elements from one batch entr
  * 1024. scale in [2^-20, 2^20].
  * lengths [B]: keys j >= lengths[b] are not seen, nor read (NULL: all of Tk). q_lengths [B]: rows i >= q_lengths[b]
  * give zeros and take no gradient (NULL: all). q_start [B] (NULL: 0). Rows that see no key give zeros. lengths are
- * clamped to [0, Tk] / [0, Tq].
+ * clamped to [0, Tk] / [0, Tq]. Keys past the last query of a causal entry are not read either. An infinity or NaN in v
+ * may reach rows of its batch entry and head that see other keys only.
  * lse: NULL, or [B,Hq,Tq] fp32 for the backward: log2 of the row's sum of exponentials (+inf: no key).
  * backward: writes dq, dk, dv (any strides, channels contiguous) and dtable [n_buckets][Hq] from the forward's
  * arguments, its out and lse, and dout. Every sum runs in a fixed order: results repeat bit for bit.
